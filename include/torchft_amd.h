@@ -12,7 +12,8 @@
  *   - return 0 on success, a negative tft_status on error; tft_last_error()
  *     returns a thread-local message for the last failing call on this thread;
  *   - the library never allocates device memory and never synchronises: each
- *     call validates its arguments on the host and enqueues exactly one kernel on
+ *     call validates its arguments on the host and enqueues exactly one kernel (the
+ *     activation entries at the end: up to three, one behind the other) on
  *     the caller's hipStream_t (passed as void*; NULL is the legacy default
  *     stream).  Mutable state: the error string (thread-local), and for
  *     tft_mt_diloco_outer_noalloc alone a fixed device array owned by the library
@@ -60,7 +61,7 @@
 extern "C" {
 #endif
 
-#define TFT_ABI_VERSION 6
+#define TFT_ABI_VERSION 7
 #define TFT_MAX_REPLICAS 8 /* replica pointer columns per launch */
 #define TFT_MIN_CHUNK_ELEMS 8192u
 #define TFT_NOALLOC_MAX_TENSORS 4096u /* rows of the built-in table of the allocation-free entry */
@@ -232,6 +233,76 @@ int tft_probe_rw_pair(void* a, void* scratch, uint64_t bytes, void* stream);
  * a power of two >= 16384.
  */
 int tft_mt_copy_bytes(const tft_mt_table* table, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Activations kept in 8 bits for the backward pass
+ *
+ * Packed form of a [rows, features] matrix:
+ *   values    uint8 [rows][pitch]   E4M3 numbers (OCP, no infinities); pitch is a
+ *                                   multiple of 16, not behind the last block; the
+ *                                   entries write zeros between features and pitch
+ *   exponents uint8 [rows][ceil(features / 128)]  one power of two per block of 128
+ *                                   consecutive features of a row, biased by 127
+ * An element stands for value * 2^(exponent - 127).  Packing takes the smallest exponent with
+ * max |x| <= 448 * 2^(exponent - 127) over the block's finite elements, limited to 10 .. 246,
+ * and rounds x / 2^(exponent - 127) to E4M3 (nearest even).  Infinities and NaN become NaN and
+ * leave the block's other elements as they would be without them; |x| over 448 * 2^119 becomes
+ * that, and |x| of at most 2^-127 becomes zero.  Every packed value is exact in bf16.
+ *
+ * dtype is TFT_F32, TFT_BF16 or TFT_F16 (TFT_F64 is refused).  Row strides count elements
+ * and may be any number from 0; the elements of a row are consecutive.  Sizes of zero are a
+ * successful no-op (sums over no rows are written as zeros).  `values` and workspaces start at
+ * a multiple of 16 bytes, everything else at a multiple of its element size.  The reference
+ * has no counterpart of these entries: it leaves activations to torch.
+ */
+
+/* x [rows, features] -> packed form */
+int tft_pack_e4m3(void* values, void* exponents, const void* x, int64_t rows, int64_t features,
+                  int64_t x_row_stride, int64_t pitch, int dtype, void* stream);
+
+/* packed form -> out [rows, features] (contiguous), times column_scale[features] unless that is
+ * NULL; without it a value that fp16 cannot hold becomes fp16's largest. */
+int tft_unpack_e4m3(void* out, const void* values, const void* exponents, const void* column_scale,
+                    int64_t rows, int64_t features, int64_t pitch, int scale_dtype, int dtype,
+                    void* stream);
+
+/* h = x + residual, rounded to dtype (h = x and nothing written where both are NULL);
+ * rstd = 1 / sqrt(mean(h^2) + eps) in fp32;  n = h * rstd;  y = n * weight (n where it is NULL),
+ * rounded once;  values / exponents = n packed (not where they are NULL); rstd may be NULL.
+ * features <= 16384; weight_dtype is dtype or TFT_F32; y and h are contiguous. */
+int tft_rms_norm(void* y, void* h, void* values, void* exponents, float* rstd, const void* x,
+                 const void* residual, const void* weight, int64_t rows, int64_t features,
+                 int64_t x_row_stride, int64_t residual_row_stride, int64_t pitch, float eps,
+                 int weight_dtype, int dtype, void* stream);
+
+/* With g = grad_y * weight and n the packed form:
+ *   grad_x = rstd * (g - n * mean(g * n)) + grad_h      (grad_h may be NULL)
+ *   grad_weight = sum over rows of grad_y * n           (not where it is NULL)
+ * grad_x is also the residual's gradient.  Rows are added in a fixed order. */
+int64_t tft_rms_norm_backward_workspace(int64_t rows, int64_t features);
+int tft_rms_norm_backward(void* grad_x, void* grad_weight, void* workspace, int64_t workspace_bytes,
+                          const void* grad_y, const void* grad_h, const void* values,
+                          const void* exponents, const float* rstd, const void* weight, int64_t rows,
+                          int64_t features, int64_t grad_y_row_stride, int64_t grad_h_row_stride,
+                          int64_t pitch, int weight_dtype, int dtype, void* stream);
+
+/* out[columns] = sum over rows of x, in fp32, rounded once, in a fixed order (a bias's gradient) */
+int64_t tft_column_sum_workspace(int64_t rows, int64_t columns);
+int tft_column_sum(void* out, void* workspace, int64_t workspace_bytes, const void* x, int64_t rows,
+                   int64_t columns, int64_t x_row_stride, int out_dtype, int dtype, void* stream);
+
+/* grad_weight[o][f] = column_scale[f] * sum over rows t of grad_out[t][o] * packed[t][f]
+ * (no scale where it is NULL), [out_features, features] contiguous and starting at a multiple of
+ * 16 bytes.  Products of bf16 numbers that add up to the operands exactly, sums in fp32, rounded
+ * once.  The workspace depends on the address of grad_out by its alignment only. */
+int64_t tft_linear_weight_grad_workspace(const void* grad_out, int64_t rows, int64_t out_features,
+                                         int64_t features, int64_t grad_row_stride, int64_t pitch,
+                                         int dtype);
+int tft_linear_weight_grad(void* grad_weight, void* workspace, int64_t workspace_bytes,
+                           const void* grad_out, const void* values, const void* exponents,
+                           const void* column_scale, int64_t rows, int64_t out_features,
+                           int64_t features, int64_t grad_row_stride, int64_t pitch, int out_dtype,
+                           int scale_dtype, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

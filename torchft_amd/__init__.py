@@ -7,6 +7,7 @@ process-group plugins.  The arithmetic runs in HIP kernels behind the C ABI
 declared in ``include/torchft_amd.h``; there is no CPU fallback.
 """
 
+from .activations import PackedActivation, pack_activations
 from .checkpointing import CheckpointServer, CheckpointTransport
 from .ddp import DistributedDataParallel, GradBucketAverager, PureDistributedDataParallel
 from .local_cluster import InProcessLighthouse, ProcessGroupThreads, ThreadWorld
@@ -39,6 +40,7 @@ __all__ = (
     "ManagerClientAdapter",
     "Optimizer",
     "OptimizerWrapper",
+    "PackedActivation",
     "ProcessGroup",
     "ProcessGroupDummy",
     "ProcessGroupLocalReplicas",
@@ -49,4 +51,5 @@ __all__ = (
     "StaticQuorum",
     "ThreadWorld",
     "WorldSizeMode",
+    "pack_activations",
 )

@@ -14,12 +14,15 @@ from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
 REPO_ROOT = PKG_DIR.parent
-SRC = PKG_DIR / "csrc" / "replica_sync.hip"
+CSRC_DIR = PKG_DIR / "csrc"
+SRC = CSRC_DIR / "replica_sync.hip"
+ACTIVATIONS_SRC = CSRC_DIR / "activations.hip"
 INCLUDE_DIR = REPO_ROOT / "include"
 LIB_DIR = PKG_DIR / "lib"
 LIB_PATH = LIB_DIR / "libtorchft_amd.so"
-# same source compiled with -DTFT_TUNING: additionally exports tft_set_launch_variant and
-# instantiates every launch shape; loaded only by the test-suite and by tuning sweeps
+# the replica-sync source compiled with -DTFT_TUNING: additionally exports
+# tft_set_launch_variant and instantiates every launch shape; loaded only by the test-suite
+# and by tuning sweeps
 TUNING_LIB_PATH = LIB_DIR / "libtorchft_amd_tuning.so"
 
 # -packed-fp32-ops: keep hipcc from forming packed fp32 instructions out of the
@@ -29,7 +32,6 @@ HIPCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     "-Xclang",
     "-target-feature",
     "-Xclang",
@@ -44,15 +46,14 @@ def hipcc_path() -> str:
     return exe
 
 
-def _compile(out_path: Path, defines, verbose: bool) -> subprocess.Popen:
-    tmp = out_path.with_suffix(".so.tmp")
-    cmd = [hipcc_path(), *HIPCC_FLAGS, *defines, f"-I{INCLUDE_DIR}", str(SRC), "-o", str(tmp)]
+def _start(args, verbose: bool) -> subprocess.Popen:
+    cmd = [hipcc_path(), *args]
     if verbose:
         print("[torchft_amd] " + " ".join(cmd), flush=True)
     return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
 
 
-def _finish(proc: subprocess.Popen, out_path: Path, verbose: bool) -> None:
+def _finish(proc: subprocess.Popen, verbose: bool) -> None:
     stdout, _ = proc.communicate()
     # the host pass does not know the device-only feature flag; that warning is noise
     out = "\n".join(line for line in stdout.splitlines() if "packed-fp32-ops" not in line)
@@ -60,17 +61,30 @@ def _finish(proc: subprocess.Popen, out_path: Path, verbose: bool) -> None:
         raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{out}")
     if verbose and out.strip():
         print(out, flush=True)
-    os.replace(out_path.with_suffix(".so.tmp"), out_path)
 
 
 def build(verbose: bool = True, tuning: bool = True) -> Path:
     """Compiles the library (and its tuning twin) unconditionally; returns the library's path."""
-    LIB_DIR.mkdir(parents=True, exist_ok=True)
-    jobs = [(_compile(LIB_PATH, [], verbose), LIB_PATH)]
+    obj_dir = LIB_DIR / "build"
+    obj_dir.mkdir(parents=True, exist_ok=True)
+    sync_obj, tuning_obj = obj_dir / "replica_sync.o", obj_dir / "replica_sync_tuning.o"
+    activations_obj = obj_dir / "activations.o"
+    sources = [(SRC, sync_obj, []), (ACTIVATIONS_SRC, activations_obj, [])]
+    links = [(LIB_PATH, [sync_obj, activations_obj])]
     if tuning:
-        jobs.append((_compile(TUNING_LIB_PATH, ["-DTFT_TUNING"], verbose), TUNING_LIB_PATH))
-    for proc, path in jobs:
-        _finish(proc, path, verbose)
+        sources.append((SRC, tuning_obj, ["-DTFT_TUNING"]))
+        links.append((TUNING_LIB_PATH, [tuning_obj, activations_obj]))
+    jobs = [
+        _start([*HIPCC_FLAGS, *defines, f"-I{INCLUDE_DIR}", "-c", str(src), "-o", str(obj)], verbose)
+        for src, obj, defines in sources
+    ]
+    for proc in jobs:
+        _finish(proc, verbose)
+    for path, objects in links:
+        tmp = path.with_suffix(".so.tmp")
+        _finish(_start(["--offload-arch=gfx950", "-shared", *map(str, objects), "-o", str(tmp)], verbose),
+                verbose)
+        os.replace(tmp, path)
     return LIB_PATH
 
 

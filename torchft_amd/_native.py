@@ -18,7 +18,7 @@ import torch  # noqa: F401  (must precede loading the library, see module docstr
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libtorchft_amd.so"
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 MAX_REPLICAS = 8
 MIN_CHUNK_ELEMS = 8192
 MIN_CHUNK_BYTES = 16384  # tft_mt_copy_bytes counts bytes
@@ -88,6 +88,32 @@ SIGNATURES = {
     "tft_mt_outer_sgd_of_sum": (c_int, [POINTER(MtTable), c_uint32, c_int, POINTER(SgdParams), c_void_p]),
     "tft_mt_copy_bytes": (c_int, [POINTER(MtTable), c_void_p]),
     "tft_probe_rw_pair": (c_int, [c_void_p, c_void_p, c_uint64, c_void_p]),
+    "tft_pack_e4m3": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]
+    ),
+    "tft_unpack_e4m3": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p],
+    ),
+    "tft_rms_norm": (
+        c_int,
+        [c_void_p] * 8 + [c_int64] * 5 + [c_float, c_int, c_int, c_void_p],
+    ),
+    "tft_rms_norm_backward_workspace": (c_int64, [c_int64, c_int64]),
+    "tft_rms_norm_backward": (
+        c_int,
+        [c_void_p] * 3 + [c_int64] + [c_void_p] * 6 + [c_int64] * 5 + [c_int, c_int, c_void_p],
+    ),
+    "tft_column_sum_workspace": (c_int64, [c_int64, c_int64]),
+    "tft_column_sum": (
+        c_int,
+        [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p],
+    ),
+    "tft_linear_weight_grad_workspace": (c_int64, [c_void_p] + [c_int64] * 5 + [c_int]),
+    "tft_linear_weight_grad": (
+        c_int,
+        [c_void_p, c_void_p, c_int64] + [c_void_p] * 4 + [c_int64] * 5 + [c_int] * 3 + [c_void_p],
+    ),
 }
 
 

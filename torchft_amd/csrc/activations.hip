@@ -1,0 +1,1317 @@
+// Activations kept in 8 bits for the backward pass (gfx950): packing, the root-mean-square
+// norm that writes its normalised rows packed, that norm's gradients, and a linear layer's
+// weight gradient from a packed input.
+//
+// The packed form of a row is E4M3 numbers with one power-of-two scale 2^k for every block of
+// 128 consecutive features, k the smallest integer with max |x| <= 448 * 2^k in the block.
+// A scale that is a power of two makes the scaling exact in both directions, the scale one
+// byte, and every packed value exact in bf16 (4 significant bits, exponents -126 .. 127).
+//
+// A block is 16 lanes of 8 features each: one DPP row of a wavefront, so the block maximum is
+// four row rotations and needs neither LDS nor a barrier.
+//
+// Entry points are declared and documented in include/torchft_amd.h.
+
+#include <hip/hip_runtime.h>
+#include <hip/hip_fp16.h>
+#include <stdint.h>
+
+#include "errors.h"
+#include "torchft_amd.h"
+
+namespace {
+
+using tft::fail;
+
+constexpr int kBlock = 128;      // features that share a scale
+constexpr int kMinExponent = 10;   // 2^-117: times E4M3's least step 2^-9 still a normal bf16
+constexpr int kMaxExponent = 246;  // 2^119: times 448 still finite in bf16
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));  // rows start where they start: gfx950 loads
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));  // 128 bits from any address
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+// ---------------------------------------------------------------------------
+// Element types: eight consecutive elements of a row as fp32
+// ---------------------------------------------------------------------------
+struct F32 {
+  typedef float elem_t;
+  typedef struct { u32x4 w[2]; } raw_t;
+  __device__ static inline raw_t load(const elem_t* p) {
+    raw_t r;
+    r.w[0] = *reinterpret_cast<const u32x4_a4*>(p);
+    r.w[1] = *reinterpret_cast<const u32x4_a4*>(p + 4);
+    return r;
+  }
+  __device__ static inline void widen(const raw_t& r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r.w[i >> 2][i & 3]);
+  }
+  __device__ static inline raw_t narrow(const float (&v)[8]) {
+    raw_t r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.w[i >> 2][i & 3] = __float_as_uint(v[i]);
+    return r;
+  }
+  __device__ static inline void store(elem_t* p, const raw_t& r) {
+    *reinterpret_cast<u32x4_a4*>(p) = r.w[0];
+    *reinterpret_cast<u32x4_a4*>(p + 4) = r.w[1];
+  }
+  __device__ static inline float widen1(elem_t x) { return x; }
+  __device__ static inline elem_t narrow1(float x) { return x; }
+  // a packed value as this type: every one of them is an fp32 number
+  __device__ static inline float in_range(float x) { return x; }
+};
+
+struct BF16 {
+  typedef uint16_t elem_t;
+  typedef struct { u32x4 w[1]; } raw_t;
+  __device__ static inline raw_t load(const elem_t* p) {
+    raw_t r;
+    r.w[0] = *reinterpret_cast<const u32x4_a2*>(p);
+    return r;
+  }
+  __device__ static inline void widen(const raw_t& r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(r.w[0][i] << 16);
+      v[2 * i + 1] = __uint_as_float(r.w[0][i] & 0xffff0000u);
+    }
+  }
+  __device__ static inline raw_t narrow(const float (&v)[8]) {
+    raw_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x2 pair = {v[2 * i], v[2 * i + 1]};
+      r.w[0][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, bf16x2));
+    }
+    return r;
+  }
+  __device__ static inline void store(elem_t* p, const raw_t& r) {
+    *reinterpret_cast<u32x4_a2*>(p) = r.w[0];
+  }
+  __device__ static inline float widen1(elem_t x) { return __uint_as_float((uint32_t)x << 16); }
+  __device__ static inline elem_t narrow1(float x) {
+    return __builtin_bit_cast(uint16_t, (__bf16)x);
+  }
+  __device__ static inline float in_range(float x) { return x; }
+};
+
+struct F16 {
+  typedef uint16_t elem_t;
+  typedef struct { u32x4 w[1]; } raw_t;
+  __device__ static inline raw_t load(const elem_t* p) {
+    raw_t r;
+    r.w[0] = *reinterpret_cast<const u32x4_a2*>(p);
+    return r;
+  }
+  __device__ static inline float widen1(elem_t x) { return __half2float(__ushort_as_half(x)); }
+  __device__ static inline elem_t narrow1(float x) {
+    // keeps the compiler from folding a multiply-add into the conversion, which would round
+    // once where the fp32 result rounds first
+    asm volatile("" : "+v"(x));
+    return __half_as_ushort(__float2half_rn(x));
+  }
+  __device__ static inline void widen(const raw_t& r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = widen1((uint16_t)(r.w[0][i] & 0xffffu));
+      v[2 * i + 1] = widen1((uint16_t)(r.w[0][i] >> 16));
+    }
+  }
+  __device__ static inline raw_t narrow(const float (&v)[8]) {
+    raw_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r.w[0][i] = (uint32_t)narrow1(v[2 * i]) | ((uint32_t)narrow1(v[2 * i + 1]) << 16);
+    return r;
+  }
+  __device__ static inline void store(elem_t* p, const raw_t& r) {
+    *reinterpret_cast<u32x4_a2*>(p) = r.w[0];
+  }
+  // a packed value may have been rounded up past fp16's largest number
+  __device__ static inline float in_range(float x) {
+    return fabsf(x) > 65504.0f ? copysignf(65504.0f, x) : x;  // NaN stays NaN
+  }
+};
+
+// Elements n .. 7 of the eight lie behind the row's end: they are not touched and count as zero.
+template <typename T>
+__device__ inline typename T::raw_t load_row(const typename T::elem_t* p, int n) {
+  if (n >= 8) return T::load(p);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = i < n ? T::widen1(p[i]) : 0.0f;
+  return T::narrow(v);
+}
+
+template <typename T>
+__device__ inline void store_row(typename T::elem_t* p, const float (&v)[8], int n) {
+  const typename T::raw_t r = T::narrow(v);
+  if (n >= 8) {
+    T::store(p, r);
+    return;
+  }
+  constexpr int kPerWord = 4 / sizeof(typename T::elem_t);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) {
+      const uint32_t word = r.w[(i / kPerWord) >> 2][(i / kPerWord) & 3];
+      if constexpr (kPerWord == 1) p[i] = __uint_as_float(word);
+      else p[i] = (typename T::elem_t)(word >> (16 * (i & 1)));
+    }
+}
+
+// Weights are given in the activations' type or in fp32.
+template <typename T>
+__device__ inline void load_weight(const void* w, bool is_f32, int64_t col, int n, float (&v)[8]) {
+  if (is_f32) {
+    F32::widen(load_row<F32>(static_cast<const float*>(w) + col, n), v);
+  } else {
+    T::widen(load_row<T>(static_cast<const typename T::elem_t*>(w) + col, n), v);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Reductions over lanes
+// ---------------------------------------------------------------------------
+template <int N>
+__device__ inline uint32_t row_rotate(uint32_t x) {  // within the 16 lanes of a DPP row
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + N, 0xf, 0xf, false);
+}
+
+__device__ inline uint32_t max_of_16(uint32_t x) {
+  x = max(x, row_rotate<8>(x));
+  x = max(x, row_rotate<4>(x));
+  x = max(x, row_rotate<2>(x));
+  return max(x, row_rotate<1>(x));
+}
+
+__device__ inline float sum_of_wave(float x) {
+  x += __uint_as_float(row_rotate<8>(__float_as_uint(x)));
+  x += __uint_as_float(row_rotate<4>(__float_as_uint(x)));
+  x += __uint_as_float(row_rotate<2>(__float_as_uint(x)));
+  x += __uint_as_float(row_rotate<1>(__float_as_uint(x)));
+  x += __shfl_xor(x, 16, 64);
+  x += __shfl_xor(x, 32, 64);
+  return x;
+}
+
+// Sum over the W wavefronts of a team; every lane gets it.  `part` holds W floats of LDS and
+// must not be in use from an earlier call (the caller alternates between two).
+template <int W>
+__device__ inline float sum_of_team(float x, float* part) {
+  x = sum_of_wave(x);
+  if constexpr (W > 1) {
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = part[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) x += part[i];
+  }
+  return x;
+}
+
+// ---------------------------------------------------------------------------
+// E4M3 with a power-of-two scale
+// ---------------------------------------------------------------------------
+__device__ inline uint32_t max_bits(const float (&v)[8]) {  // bits of max |v|; NaN counts as most
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+
+__device__ inline int exponent_for(uint32_t bits) {
+  // (bits + 0x1fffff) >> 23 is the exponent of bits, one more where the significand is over
+  // 1.75 = 448 / 2^8
+  const int e = (int)((bits + 0x1fffffu) >> 23) - 8;
+  return min(max(e, kMinExponent), kMaxExponent);
+}
+
+// Eight values of one lane of a block's sixteen -> 8 bytes and the block's biased exponent.
+// All sixteen lanes call it together.
+__device__ inline u32x2 quantise(float (&v)[8], int* exponent) {
+  uint32_t top = max_of_16(max_bits(v));
+  constexpr uint32_t kMost = ((uint32_t)(kMaxExponent + 8) << 23) | 0x600000u;  // 448 * 2^119
+  if (top > kMost) {  // the same for all sixteen: infinities, NaN or next to fp32's largest
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+      if (b >= kInfBits) v[i] = __uint_as_float(0x7fc00000u);  // E4M3 has a NaN and no infinity
+      else m = max(m, b);
+    }
+    top = max_of_16(m);
+    const float most = __uint_as_float(kMost);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (fabsf(v[i]) > most) v[i] = copysignf(most, v[i]);
+  }
+  *exponent = exponent_for(top);
+  const float inverse = __uint_as_float((uint32_t)(254 - *exponent) << 23);
+  u32x2 q;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] * inverse, v[4 * i + 1] * inverse, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] * inverse, v[4 * i + 3] * inverse, w, true);
+    q[i] = (uint32_t)w;
+  }
+  return q;
+}
+
+__device__ inline float scale_of(uint32_t exponent) { return __uint_as_float(exponent << 23); }
+
+__device__ inline void dequantise(const u32x2& q, float scale, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[i], false);
+    const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[i], true);
+    v[4 * i] = lo[0] * scale;
+    v[4 * i + 1] = lo[1] * scale;
+    v[4 * i + 2] = hi[0] * scale;
+    v[4 * i + 3] = hi[1] * scale;
+  }
+}
+
+// n / d for n < 2^31 by a multiplication (d >= 1)
+struct Divider {
+  uint32_t d, magic, shift;
+};
+
+Divider make_divider(uint32_t d) {
+  uint32_t s = 0;
+  while ((1ull << s) < d) ++s;
+  return {d, (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
+}
+
+__device__ inline uint32_t divide(uint32_t n, const Divider& d) {
+  return (__umulhi(n, d.magic) + n) >> d.shift;
+}
+
+// ---------------------------------------------------------------------------
+// Pack and unpack
+// ---------------------------------------------------------------------------
+struct PackArgs {
+  const void* x;
+  uint8_t* values;
+  uint8_t* exponents;
+  int64_t features, row_stride, pitch;
+  uint32_t blocks;  // of all rows
+  Divider per_row;
+};
+
+constexpr int kPackThreads = 256;
+constexpr int kPackUnroll = 4;
+constexpr int kPackBlocks = kPackThreads / 16 * kPackUnroll;  // blocks per workgroup
+
+template <typename T>
+__global__ __launch_bounds__(kPackThreads) void pack_kernel(PackArgs a) {
+  const int lane = threadIdx.x & 15;
+  const uint32_t first = blockIdx.x * (uint32_t)kPackBlocks + (threadIdx.x >> 4);
+  const typename T::elem_t* x = static_cast<const typename T::elem_t*>(a.x);
+  typename T::raw_t raw[kPackUnroll];
+  uint32_t row[kPackUnroll];
+  int64_t col[kPackUnroll];
+#pragma unroll
+  for (int u = 0; u < kPackUnroll; ++u) {
+    const uint32_t b = first + u * (kPackThreads / 16);
+    row[u] = divide(min(b, a.blocks - 1), a.per_row);
+    col[u] = (int64_t)(min(b, a.blocks - 1) - row[u] * a.per_row.d) * kBlock + lane * 8;
+    const int64_t left = b < a.blocks ? a.features - col[u] : 0;
+    raw[u] = load_row<T>(x + (int64_t)row[u] * a.row_stride + col[u], (int)min(left, (int64_t)8));
+  }
+#pragma unroll
+  for (int u = 0; u < kPackUnroll; ++u) {
+    const uint32_t b = first + u * (kPackThreads / 16);
+    if (b >= a.blocks) return;  // the same for a block's sixteen lanes
+    float v[8];
+    T::widen(raw[u], v);
+    int e;
+    const u32x2 q = quantise(v, &e);
+    if (col[u] < a.pitch)
+      *reinterpret_cast<u32x2*>(a.values + (int64_t)row[u] * a.pitch + col[u]) = q;
+    if (lane == 0) a.exponents[b] = (uint8_t)e;
+  }
+}
+
+struct UnpackArgs {
+  void* out;
+  const uint8_t* values;
+  const uint8_t* exponents;
+  const void* column_scale;
+  int64_t features, pitch;
+  uint32_t blocks;
+  Divider per_row;
+};
+
+// S: type of the column scale
+template <typename T, typename S>
+__global__ __launch_bounds__(kPackThreads) void unpack_kernel(UnpackArgs a) {
+  const int lane = threadIdx.x & 15;
+  const uint32_t first = blockIdx.x * (uint32_t)kPackBlocks + (threadIdx.x >> 4);
+  typename T::elem_t* out = static_cast<typename T::elem_t*>(a.out);
+  u32x2 q[kPackUnroll];
+  uint32_t e[kPackUnroll], row[kPackUnroll];
+  int64_t col[kPackUnroll];
+#pragma unroll
+  for (int u = 0; u < kPackUnroll; ++u) {
+    const uint32_t b = min(first + u * (kPackThreads / 16), a.blocks - 1);
+    row[u] = divide(b, a.per_row);
+    col[u] = (int64_t)(b - row[u] * a.per_row.d) * kBlock + lane * 8;
+    q[u] = u32x2{0, 0};
+    if (col[u] < a.pitch)
+      q[u] = *reinterpret_cast<const u32x2*>(a.values + (int64_t)row[u] * a.pitch + col[u]);
+    e[u] = a.exponents[b];
+  }
+#pragma unroll
+  for (int u = 0; u < kPackUnroll; ++u) {
+    if (first + u * (kPackThreads / 16) >= a.blocks) return;
+    const int n = (int)min(a.features - col[u], (int64_t)8);
+    if (n <= 0) continue;
+    float v[8];
+    dequantise(q[u], scale_of(e[u]), v);
+    if (a.column_scale) {
+      float w[8];
+      load_weight<S>(a.column_scale, false, col[u], n, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= w[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = T::in_range(v[i]);
+    }
+    store_row<T>(out + (int64_t)row[u] * a.features + col[u], v, n);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Root-mean-square norm
+// ---------------------------------------------------------------------------
+struct NormArgs {
+  const void* x;
+  const void* residual;  // or NULL
+  const void* weight;    // or NULL
+  void* y;
+  void* h;               // or NULL
+  uint8_t* values;       // or NULL: nothing is packed
+  uint8_t* exponents;
+  float* rstd;           // or NULL
+  uint32_t rows;
+  int features;
+  int64_t x_stride, residual_stride, pitch;
+  int weight_is_f32;
+  float eps;
+};
+
+// One team of W wavefronts per row, C times eight features per lane: the row is read once and
+// stays in registers between the sum of squares and the outputs.  W = 1 runs four rows per
+// workgroup without a barrier.
+template <typename T, int W, int C>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_kernel(NormArgs a) {
+  constexpr int kTeam = 64 * W;
+  __shared__ float part[W];
+  typedef typename T::elem_t elem_t;
+  const int lane = W == 1 ? (threadIdx.x & 63) : threadIdx.x;
+  const uint32_t row = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (row >= a.rows) return;  // whole teams
+  const elem_t* x = static_cast<const elem_t*>(a.x) + (int64_t)row * a.x_stride;
+  float h[C][8];
+  {
+    typename T::raw_t rx[C], rr[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = (c * kTeam + lane) * 8;
+      rx[c] = load_row<T>(x + col, a.features - col);
+    }
+    if (a.residual) {
+      const elem_t* r = static_cast<const elem_t*>(a.residual) + (int64_t)row * a.residual_stride;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int col = (c * kTeam + lane) * 8;
+        rr[c] = load_row<T>(r + col, a.features - col);
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int col = (c * kTeam + lane) * 8;
+        float s[8];
+        T::widen(rx[c], h[c]);
+        T::widen(rr[c], s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[c][i] += s[i];
+        // what is normed is the sum as it is stored: the layer's other readers see that one
+        T::widen(T::narrow(h[c]), h[c]);
+        if (col < a.features)
+          store_row<T>(static_cast<elem_t*>(a.h) + (int64_t)row * a.features + col, h[c],
+                       a.features - col);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c) T::widen(rx[c], h[c]);
+    }
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(h[c][i], h[c][i], ss);
+  ss = sum_of_team<W>(ss, part);
+  const float rstd = 1.0f / sqrtf(ss / (float)a.features + a.eps);
+  if (a.rstd && lane == 0) a.rstd[row] = rstd;
+  const int blocks = (a.features + kBlock - 1) / kBlock;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int col = (c * kTeam + lane) * 8;
+    if (col - (lane & 15) * 8 >= a.features) return;  // whole blocks
+    const int n = a.features - col;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[c][i] *= rstd;
+    if (a.weight) {
+      load_weight<T>(a.weight, a.weight_is_f32, col, n, y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] *= h[c][i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = h[c][i];
+    }
+    if (n > 0) store_row<T>(static_cast<elem_t*>(a.y) + (int64_t)row * a.features + col, y, n);
+    if (a.values) {
+      if (n < 8) {  // 0 times an infinite rstd is no zero
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i >= n) h[c][i] = 0.0f;
+      }
+      int e;
+      const u32x2 q = quantise(h[c], &e);
+      if (col < a.pitch)
+        *reinterpret_cast<u32x2*>(a.values + (int64_t)row * a.pitch + col) = q;
+      if ((lane & 15) == 0) a.exponents[(int64_t)row * blocks + col / kBlock] = (uint8_t)e;
+    }
+  }
+}
+
+struct NormBackArgs {
+  const void* grad_y;
+  const void* grad_h;  // or NULL
+  const uint8_t* values;
+  const uint8_t* exponents;
+  const float* rstd;
+  const void* weight;  // or NULL
+  void* grad_x;
+  float* partial;      // [gridDim.x][features], or NULL: no weight gradient
+  uint32_t rows;
+  int features;
+  int64_t grad_y_stride, grad_h_stride, pitch;
+  int weight_is_f32;
+};
+
+// The workgroup takes rows blockIdx.x, + gridDim.x, ... (four at a time for W = 1) and keeps the
+// weight gradient of its rows in registers; column_reduce_kernel adds the workgroups' partial
+// sums in a fixed order.
+template <typename T, int W, int C>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_back_kernel(NormBackArgs a) {
+  constexpr int kTeam = 64 * W;
+  constexpr int kRows = W == 1 ? 4 : 1;
+  __shared__ float part[2][W];
+  __shared__ float gathered[W == 1 ? 3 : 1][W == 1 ? 64 * C * 8 : 1];
+  typedef typename T::elem_t elem_t;
+  const int lane = W == 1 ? (threadIdx.x & 63) : threadIdx.x;
+  const int team = W == 1 ? (threadIdx.x >> 6) : 0;
+  const int blocks = (a.features + kBlock - 1) / kBlock;
+  const float inv_n = 1.0f / (float)a.features;
+  float gw[C][8];
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) gw[c][i] = 0.0f;
+  int turn = 0;
+  for (uint32_t row = blockIdx.x * kRows + team; row < a.rows; row += gridDim.x * kRows, turn ^= 1) {
+    typename T::raw_t rg[C];
+    u32x2 rq[C];
+    uint32_t re[C];
+    const elem_t* gy = static_cast<const elem_t*>(a.grad_y) + (int64_t)row * a.grad_y_stride;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = (c * kTeam + lane) * 8;
+      rg[c] = load_row<T>(gy + col, a.features - col);
+      rq[c] = u32x2{0, 0};
+      re[c] = 0;
+      if (col < a.pitch) {
+        rq[c] = *reinterpret_cast<const u32x2*>(a.values + (int64_t)row * a.pitch + col);
+        if (col < a.features) re[c] = a.exponents[(int64_t)row * blocks + col / kBlock];
+      }
+    }
+    const float rstd = a.rstd[row];
+    float n[C][8], g[C][8];
+    float dot = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = (c * kTeam + lane) * 8;
+      float gyv[8];
+      dequantise(rq[c], scale_of(re[c]), n[c]);
+      if (a.features - col < 8) {  // what a caller's padding holds does not count
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i >= a.features - col) n[c][i] = 0.0f;
+      }
+      T::widen(rg[c], gyv);
+      if (a.weight && col < a.features) {
+        load_weight<T>(a.weight, a.weight_is_f32, col, a.features - col, g[c]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[c][i] *= gyv[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[c][i] = gyv[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        gw[c][i] = fmaf(gyv[i], n[c][i], gw[c][i]);
+        dot = fmaf(g[c][i], n[c][i], dot);
+      }
+    }
+    dot = sum_of_team<W>(dot, part[turn]) * inv_n;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = (c * kTeam + lane) * 8;
+      if (col >= a.features) break;
+      float gx[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) gx[i] = rstd * fmaf(-n[c][i], dot, g[c][i]);
+      if (a.grad_h) {
+        float gh[8];
+        T::widen(load_row<T>(static_cast<const elem_t*>(a.grad_h) +
+                                 (int64_t)row * a.grad_h_stride + col,
+                             a.features - col),
+                 gh);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) gx[i] += gh[i];
+      }
+      store_row<T>(static_cast<elem_t*>(a.grad_x) + (int64_t)row * a.features + col, gx,
+                   a.features - col);
+    }
+  }
+  if (!a.partial) return;
+  if constexpr (W == 1) {  // the four wavefronts' sums, in their order
+    if (team) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) gathered[team - 1][(c * 8 + i) * 64 + lane] = gw[c][i];
+    }
+    __syncthreads();
+    if (team) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int t = 0; t < 3; ++t) gw[c][i] += gathered[t][(c * 8 + i) * 64 + lane];
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int col = (c * kTeam + lane) * 8;
+    if (col >= a.features) break;
+    store_row<F32>(a.partial + (int64_t)blockIdx.x * a.features + col, gw[c], a.features - col);
+  }
+}
+
+// out[c] = sum over g of partial[g][c], g in fixed order: 32 columns and 32 row lanes per
+// workgroup, the row lanes joined through LDS.
+template <typename T>
+__global__ __launch_bounds__(1024) void column_reduce_kernel(const float* partial, void* out,
+                                                             uint32_t groups, int64_t columns) {
+  __shared__ float part[32][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t col = (int64_t)blockIdx.x * 32 + x;
+  float s = 0.0f;
+  if (col < columns)
+#pragma unroll 8
+    for (uint32_t g = y; g < groups; g += 32) s += partial[(int64_t)g * columns + col];
+  part[y][x] = s;
+  __syncthreads();
+  if (y || col >= columns) return;
+#pragma unroll
+  for (int i = 1; i < 32; ++i) s += part[i][x];
+  static_cast<typename T::elem_t*>(out)[col] = T::narrow1(s);
+}
+
+// Partial column sums of a [rows, columns] matrix: 256 lanes of eight columns, rows
+// blockIdx.y, + gridDim.y, ...
+template <typename T>
+__global__ __launch_bounds__(256) void column_sum_kernel(const void* x, float* partial, uint32_t rows,
+                                                         int64_t columns, int64_t stride) {
+  const int64_t col = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (col >= columns) return;
+  const int n = (int)min(columns - col, (int64_t)8);
+  const typename T::elem_t* p = static_cast<const typename T::elem_t*>(x) + col;
+  float s[8] = {};
+#pragma unroll 4
+  for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    float v[8];
+    T::widen(load_row<T>(p + (int64_t)r * stride, n), v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] += v[i];
+  }
+  store_row<F32>(partial + (int64_t)blockIdx.y * columns + col, s, n);
+}
+
+// ---------------------------------------------------------------------------
+// Weight gradient of a linear layer:  G[o][f] = w[f] * sum_t D[t][o] X[t][f]
+// ---------------------------------------------------------------------------
+// The products run on the bf16 matrix cores.  X is exact in bf16, and D is split into bf16
+// parts that add up to it exactly: one part for bf16, two for fp16 (11 bits), three for fp32
+// (24 bits).  The parts lie behind one another along t, so the kernel sees one longer sum.
+// Written where D is not bf16 already, or its rows do not start at 16-byte boundaries.
+struct SplitArgs {
+  const void* d;
+  uint16_t* parts;  // [n_parts][rows][padded]
+  int64_t rows, columns, stride, padded;
+  uint64_t chunks;  // rows * padded / 8
+};
+
+template <typename T, int P>
+__global__ __launch_bounds__(256) void split_kernel(SplitArgs a) {
+  const int64_t per_row = a.padded / 8;
+  for (uint64_t c = blockIdx.x * 256ull + threadIdx.x; c < a.chunks; c += gridDim.x * 256ull) {
+    const int64_t row = (int64_t)(c / (uint64_t)per_row);
+    const int64_t col = (int64_t)(c - (uint64_t)row * per_row) * 8;
+    float v[8];
+    T::widen(load_row<T>(static_cast<const typename T::elem_t*>(a.d) + row * a.stride + col,
+                         (int)min(a.columns - col, (int64_t)8)),
+             v);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      u32x4 w;
+      uint32_t b[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        // cut, not rounded: what is left over is exact, and nothing is rounded to infinity
+        b[i] = __float_as_uint(v[i]);
+        const float cut = __uint_as_float(b[i] & 0xffff0000u);
+        v[i] = (b[i] & 0x7fffffffu) == kInfBits ? 0.0f : v[i] - cut;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = (b[2 * i] >> 16) | (b[2 * i + 1] & 0xffff0000u);
+      *reinterpret_cast<u32x4*>(a.parts + ((int64_t)p * a.rows + row) * a.padded + col) = w;
+    }
+  }
+}
+
+constexpr int kStep = 64;  // tokens per step of the product
+
+struct WgradArgs {
+  const uint16_t* d;  // bf16 parts [n_parts][rows][d_stride]
+  const uint8_t* values;
+  const uint8_t* exponents;
+  const void* column_scale;  // or NULL
+  void* out;                 // [out_features][features], or fp32 [splits][out_features][pitch]
+  int64_t rows, d_stride, pitch;
+  uint32_t out_features, features, blocks;
+  uint32_t tiles_o, tiles_f, splits;
+  uint32_t steps_per_part, steps;  // of all parts
+  int scale_type, out_type;        // TFT_F32 ...
+  int to_partial;
+};
+
+__device__ inline __amdgpu_buffer_rsrc_t buffer(const void* base, int64_t bytes) {
+  // reads behind the end give zero
+  const int n = (int)max((int64_t)0, min(bytes, (int64_t)0x7fffffff));
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, n, 0x00020000);
+}
+
+__device__ inline void store_out(void* out, int type, int64_t at, float v) {
+  if (type == TFT_F32) static_cast<float*>(out)[at] = v;
+  else if (type == TFT_BF16) static_cast<uint16_t*>(out)[at] = BF16::narrow1(v);
+  else static_cast<uint16_t*>(out)[at] = F16::narrow1(v);
+}
+
+__device__ inline float load_scale(const void* p, int type, int64_t at) {
+  if (type == TFT_F32) return static_cast<const float*>(p)[at];
+  if (type == TFT_BF16) return BF16::widen1(static_cast<const uint16_t*>(p)[at]);
+  return F16::widen1(static_cast<const uint16_t*>(p)[at]);
+}
+
+// Four neighbouring features of one output row, scaled and rounded
+__device__ inline void store_out4(const WgradArgs& a, int64_t o, int64_t f, f32x4 v) {
+  const int n = (int)min((int64_t)a.features - f, (int64_t)4);
+  if (a.column_scale) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) v[i] *= load_scale(a.column_scale, a.scale_type, f + i);
+  }
+  const int64_t at = o * a.features + f;
+  if (n == 4 && a.features % 4 == 0) {
+    if (a.out_type == TFT_F32) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = v;
+    } else {
+      uint16_t b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        b[i] = a.out_type == TFT_BF16 ? BF16::narrow1(v[i]) : F16::narrow1(v[i]);
+      u32x2 w = {b[0] | ((uint32_t)b[1] << 16), b[2] | ((uint32_t)b[3] << 16)};
+      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at) = w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) store_out(a.out, a.out_type, at + i, v[i]);
+}
+
+// Tile of O output rows x F features, wavefronts in a WO x WF grid.
+//
+// Both operands lie with the summed axis (tokens) outermost, so LDS holds a step's tiles as they
+// lie in memory, [token][column], and the transposing LDS reads (ds_read_b64_tr_b16: 16 lanes
+// fetch 4 tokens x 16 columns, lane i gets column i's four tokens) turn them into matrix
+// operands.  A lane's eight tokens of a 32-token product are 4g + 0..3 and 16 + 4g + 0..3 for
+// lane group g, the same in both operands.  Rows of a tile are 16-column units of 32 bytes; unit
+// u of token t lies at u ^ (t & 7), which spreads the four rows of a transposing read, and the
+// rows of two neighbouring lane groups, over all banks.
+template <int O, int F, int WO, int WF>
+__global__ __launch_bounds__(64 * WO * WF) void wgrad_kernel(WgradArgs a) {
+  constexpr int kThreads = 64 * WO * WF;
+  constexpr int kDChunks = kStep * O / 8 / kThreads;   // 16-byte chunks of D per thread and step
+  constexpr int kXChunks = kStep * F / 16 / kThreads;  // 16-byte chunks of X
+  constexpr int kFragO = O / WO / 16, kFragF = F / WF / 16;
+  __shared__ __attribute__((aligned(128))) uint16_t lds_d[2][kStep * O];
+  __shared__ __attribute__((aligned(128))) uint16_t lds_x[2][kStep * F];
+
+  const uint32_t tiles = a.tiles_o * a.tiles_f;
+  const uint32_t split = blockIdx.x / tiles;
+  const uint32_t tile = blockIdx.x - split * tiles;
+  const int64_t o0 = (int64_t)(tile / a.tiles_f) * O;
+  const int64_t f0 = (int64_t)(tile % a.tiles_f) * F;
+  const uint32_t step_begin = (uint32_t)((uint64_t)a.steps * split / a.splits);
+  const uint32_t step_end = (uint32_t)((uint64_t)a.steps * (split + 1) / a.splits);
+
+  // what this thread stages, the same in every step but for the token offset
+  uint32_t d_off[kDChunks], d_lds[kDChunks], x_off[kXChunks], x_lds[kXChunks], e_off[kXChunks];
+#pragma unroll
+  for (int i = 0; i < kDChunks; ++i) {
+    const int c = i * kThreads + threadIdx.x, t = c / (O / 8), j = c % (O / 8);
+    d_off[i] = o0 + j * 8 < a.out_features ? (uint32_t)((t * a.d_stride + j * 8) * 2) : 0x80000000u;
+    d_lds[i] = t * O + (((j >> 1) ^ (t & 7)) << 4) + ((j & 1) << 3);
+  }
+#pragma unroll
+  for (int i = 0; i < kXChunks; ++i) {
+    const int c = i * kThreads + threadIdx.x, t = c / (F / 16), u = c % (F / 16);
+    x_off[i] = f0 + u * 16 < a.pitch ? (uint32_t)(t * a.pitch + u * 16) : 0x80000000u;
+    e_off[i] = f0 + u * 16 < a.pitch ? (uint32_t)(t * a.blocks + (u * 16) / kBlock) : 0x80000000u;
+    x_lds[i] = t * F + ((u ^ (t & 7)) << 4);
+  }
+  // what this lane reads: token 4g + i / 4 (+ 16, + 32 ...), columns 4 (i % 4) .. of unit u
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int t_lane = ((lane >> 4) << 2) + ((lane & 15) >> 2);
+  const int wave_o = (wave / WF) * (O / WO), wave_f = (wave % WF) * (F / WF);
+  uint32_t d_read[kFragO], x_read[kFragF];
+#pragma unroll
+  for (int f = 0; f < kFragO; ++f)
+    d_read[f] = t_lane * O + (((wave_o / 16 + f) ^ (t_lane & 7)) << 4) + ((lane & 3) << 2);
+#pragma unroll
+  for (int f = 0; f < kFragF; ++f)
+    x_read[f] = t_lane * F + (((wave_f / 16 + f) ^ (t_lane & 7)) << 4) + ((lane & 3) << 2);
+
+  u32x4 d_reg[kDChunks], x_reg[kXChunks];
+  uint32_t e_reg[kXChunks];
+  auto fetch = [&](uint32_t step) {
+    const uint32_t part = step / a.steps_per_part;
+    const int64_t t0 = (int64_t)(step - part * a.steps_per_part) * kStep;
+    const int64_t left = a.rows - t0;
+    const auto d = buffer(a.d + ((int64_t)part * a.rows + t0) * a.d_stride + o0,
+                          (left * a.d_stride - o0) * 2);
+    const auto x = buffer(a.values + t0 * a.pitch + f0, left * a.pitch - f0);
+    const auto e = buffer(a.exponents + t0 * a.blocks + f0 / kBlock, left * a.blocks - f0 / kBlock);
+#pragma unroll
+    for (int i = 0; i < kDChunks; ++i)
+      d_reg[i] = __builtin_amdgcn_raw_buffer_load_b128(d, d_off[i], 0, 0);
+#pragma unroll
+    for (int i = 0; i < kXChunks; ++i) {
+      x_reg[i] = __builtin_amdgcn_raw_buffer_load_b128(x, x_off[i], 0, 0);
+      e_reg[i] = __builtin_amdgcn_raw_buffer_load_b8(e, e_off[i], 0, 0);
+    }
+  };
+  auto stage = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < kDChunks; ++i)
+      *reinterpret_cast<u32x4*>(&lds_d[buf][d_lds[i]]) = d_reg[i];
+    const int swap = (lane >> 2) & 1;  // lanes 4 .. 7 of eight write their halves the other way round
+#pragma unroll
+    for (int i = 0; i < kXChunks; ++i) {
+      const float scale = scale_of(e_reg[i]);
+      u32x4 half[2];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        half[w >> 1][(w & 1) * 2] = __builtin_bit_cast(
+            uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x_reg[i][w], scale, false));
+        half[w >> 1][(w & 1) * 2 + 1] = __builtin_bit_cast(
+            uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x_reg[i][w], scale, true));
+      }
+      *reinterpret_cast<u32x4*>(&lds_x[buf][x_lds[i] + swap * 8]) = swap ? half[1] : half[0];
+      *reinterpret_cast<u32x4*>(&lds_x[buf][x_lds[i] + 8 - swap * 8]) = swap ? half[0] : half[1];
+    }
+  };
+
+  f32x4 acc[kFragF][kFragO];
+#pragma unroll
+  for (int i = 0; i < kFragF; ++i)
+#pragma unroll
+    for (int j = 0; j < kFragO; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+  auto read_tr = [&](const uint16_t* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(const_cast<uint16_t*>(p)));
+  };
+  auto operand = [&](const uint16_t* base, int columns) {  // 32 tokens of one unit
+    const s16x4 lo = read_tr(base), hi = read_tr(base + 16 * columns);
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  auto multiply = [&](int buf) {
+#pragma unroll
+    for (int k = 0; k < kStep / 32; ++k) {
+      bf16x8 d[kFragO], x[kFragF];
+#pragma unroll
+      for (int i = 0; i < kFragF; ++i) x[i] = operand(&lds_x[buf][x_read[i] + k * 32 * F], F);
+#pragma unroll
+      for (int j = 0; j < kFragO; ++j) d[j] = operand(&lds_d[buf][d_read[j] + k * 32 * O], O);
+#pragma unroll
+      for (int i = 0; i < kFragF; ++i)
+#pragma unroll
+        for (int j = 0; j < kFragO; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], d[j], acc[i][j], 0, 0, 0);
+    }
+  };
+
+  if (step_begin < step_end) {
+    fetch(step_begin);
+    stage(0);
+    __syncthreads();
+    int buf = 0;
+    for (uint32_t s = step_begin; s < step_end; ++s, buf ^= 1) {
+      if (s + 1 < step_end) fetch(s + 1);
+      multiply(buf);
+      if (s + 1 < step_end) stage(buf ^ 1);
+      __syncthreads();
+    }
+  }
+
+  // a lane holds features 4 (lane / 16) .. + 3 of each 16, output row lane % 16
+#pragma unroll
+  for (int j = 0; j < kFragO; ++j) {
+    const int64_t o = o0 + wave_o + j * 16 + (lane & 15);
+    if (o >= a.out_features) continue;
+#pragma unroll
+    for (int i = 0; i < kFragF; ++i) {
+      const int64_t f = f0 + wave_f + i * 16 + (lane >> 4) * 4;
+      if (f >= a.features) continue;
+      if (a.to_partial) {
+        float* p = static_cast<float*>(a.out) + ((int64_t)split * a.out_features + o) * a.pitch + f;
+        *reinterpret_cast<f32x4*>(p) = acc[i][j];
+      } else {
+        store_out4(a, o, f, acc[i][j]);
+      }
+    }
+  }
+}
+
+// Joins the splits' partial products in their order.
+__global__ __launch_bounds__(256) void wgrad_join_kernel(WgradArgs a, const float* partial) {
+  const uint64_t per_row = (uint64_t)a.pitch / 4;
+  const uint64_t chunks = (uint64_t)a.out_features * per_row;
+  for (uint64_t c = blockIdx.x * 256ull + threadIdx.x; c < chunks; c += gridDim.x * 256ull) {
+    const int64_t o = (int64_t)(c / per_row), f = (int64_t)(c - (uint64_t)o * per_row) * 4;
+    if (f >= a.features) continue;
+    const float* p = partial + (int64_t)c * 4;
+    f32x4 v = *reinterpret_cast<const f32x4*>(p);
+    for (uint32_t s = 1; s < a.splits; ++s)
+      v += *reinterpret_cast<const f32x4*>(p + (int64_t)s * a.out_features * a.pitch);
+    store_out4(a, o, f, v);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+constexpr int64_t kMostRows = 1ll << 31;
+constexpr int kMostNormFeatures = 16384;
+
+bool known_type(int t) { return t == TFT_F32 || t == TFT_BF16 || t == TFT_F16; }
+
+int check_types(const char* what, int dtype, int weight_dtype, bool has_weight) {
+  if (!known_type(dtype))
+    return fail(TFT_ERR_UNSUPPORTED, "%s: dtype %d is not fp32, bf16 or fp16", what, dtype);
+  if (has_weight && !known_type(weight_dtype))
+    return fail(TFT_ERR_UNSUPPORTED, "%s: weight dtype %d is not fp32, bf16 or fp16", what, weight_dtype);
+  return TFT_OK;
+}
+
+// Common checks of a packed matrix; `rows` and `features` at least 1 behind this.
+int check_packed(const char* what, const void* values, const void* exponents, int64_t rows,
+                 int64_t features, int64_t pitch) {
+  if (rows >= kMostRows) return fail(TFT_ERR_UNSUPPORTED, "%s: %lld rows, at most 2^31 - 1", what, (long long)rows);
+  if (features >= kMostRows)
+    return fail(TFT_ERR_UNSUPPORTED, "%s: %lld features, at most 2^31 - 1", what, (long long)features);
+  if (pitch < features || pitch % 16 || pitch >= features + kBlock)
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: pitch %lld does not fit %lld features (a multiple of 16, less than 128 more)",
+                what, (long long)pitch, (long long)features);
+  const int64_t blocks = (features + kBlock - 1) / kBlock;
+  if (pitch > blocks * kBlock)
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: pitch %lld lies behind the last block of %lld features", what,
+                (long long)pitch, (long long)features);
+  if (rows * blocks >= (1ll << 31))
+    return fail(TFT_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 blocks of 128 features", what);
+  if (!values || !exponents) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: packed buffers are NULL", what);
+  if (reinterpret_cast<uintptr_t>(values) & 15u)
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: packed values must start at a multiple of 16 bytes", what);
+  return TFT_OK;
+}
+
+int esize(int dtype) { return dtype == TFT_F32 ? 4 : 2; }
+
+bool misaligned(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(esize(dtype) - 1)) != 0; }
+
+int launch(const char* what, const void* kernel, dim3 grid, int threads, void** params, hipStream_t s) {
+  const hipError_t e = hipLaunchKernel(kernel, grid, dim3(threads), params, 0, s);
+  if (e != hipSuccess) return fail(TFT_ERR_LAUNCH, "%s: launch failed: %s", what, hipGetErrorString(e));
+  return TFT_OK;
+}
+
+#define TFT_KERNEL(...) reinterpret_cast<const void*>(&__VA_ARGS__)
+
+template <typename T>
+int launch_norm(const char* what, const NormArgs& a, hipStream_t s) {
+  NormArgs args = a;
+  void* params[] = {&args};
+  const dim3 four((a.rows + 3) / 4), one(a.rows);
+  if (a.features <= 512) return launch(what, TFT_KERNEL(norm_kernel<T, 1, 1>), four, 256, params, s);
+  if (a.features <= 1024) return launch(what, TFT_KERNEL(norm_kernel<T, 1, 2>), four, 256, params, s);
+  if (a.features <= 2048) return launch(what, TFT_KERNEL(norm_kernel<T, 4, 1>), one, 256, params, s);
+  if (a.features <= 4096) return launch(what, TFT_KERNEL(norm_kernel<T, 4, 2>), one, 256, params, s);
+  if (a.features <= 8192) return launch(what, TFT_KERNEL(norm_kernel<T, 4, 4>), one, 256, params, s);
+  return launch(what, TFT_KERNEL(norm_kernel<T, 8, 4>), one, 512, params, s);
+}
+
+constexpr uint32_t kNormBackGroups = 512;
+
+uint32_t norm_back_groups(int64_t rows, int64_t features) {
+  const int64_t teams = features <= 1024 ? (rows + 3) / 4 : rows;
+  return (uint32_t)(teams < (int64_t)kNormBackGroups ? teams : (int64_t)kNormBackGroups);
+}
+
+template <typename T>
+int launch_norm_back(const char* what, const NormBackArgs& a, hipStream_t s) {
+  NormBackArgs args = a;
+  void* params[] = {&args};
+  const dim3 grid(norm_back_groups(a.rows, a.features));
+  if (a.features <= 512) return launch(what, TFT_KERNEL(norm_back_kernel<T, 1, 1>), grid, 256, params, s);
+  if (a.features <= 1024) return launch(what, TFT_KERNEL(norm_back_kernel<T, 1, 2>), grid, 256, params, s);
+  if (a.features <= 2048) return launch(what, TFT_KERNEL(norm_back_kernel<T, 4, 1>), grid, 256, params, s);
+  if (a.features <= 4096) return launch(what, TFT_KERNEL(norm_back_kernel<T, 4, 2>), grid, 256, params, s);
+  if (a.features <= 8192) return launch(what, TFT_KERNEL(norm_back_kernel<T, 8, 2>), grid, 512, params, s);
+  return launch(what, TFT_KERNEL(norm_back_kernel<T, 8, 4>), grid, 512, params, s);
+}
+
+int launch_column_reduce(const char* what, const float* partial, void* out, uint32_t groups,
+                         int64_t columns, int dtype, hipStream_t s) {
+  void* params[] = {&partial, &out, &groups, &columns};
+  const dim3 grid((uint32_t)((columns + 31) / 32));
+  const void* k = dtype == TFT_F32 ? TFT_KERNEL(column_reduce_kernel<F32>)
+                  : dtype == TFT_BF16 ? TFT_KERNEL(column_reduce_kernel<BF16>)
+                                      : TFT_KERNEL(column_reduce_kernel<F16>);
+  return launch(what, k, grid, 1024, params, s);
+}
+
+uint32_t column_sum_groups(int64_t rows, int64_t columns) {
+  const int64_t across = (columns + 2047) / 2048;
+  int64_t g = (512 + across - 1) / across;
+  if (g > (rows + 7) / 8) g = (rows + 7) / 8;
+  return (uint32_t)(g < 1 ? 1 : g);
+}
+
+// How a weight gradient is cut.
+struct WgradPlan {
+  int parts;       // bf16 parts of the gradient
+  bool split_first;  // they are written to the workspace
+  int64_t padded;  // row length of the parts
+  bool large;
+  uint32_t tiles_o, tiles_f, steps_per_part, steps, splits;
+  int64_t parts_bytes, partial_bytes;
+};
+
+WgradPlan plan_wgrad(int64_t rows, int64_t out_features, int64_t features, int64_t pitch,
+                     int64_t grad_stride, int dtype, bool aligned) {
+  WgradPlan p{};
+  p.parts = dtype == TFT_F32 ? 3 : dtype == TFT_F16 ? 2 : 1;
+  p.split_first = dtype != TFT_BF16 || !aligned || out_features % 8 || grad_stride % 8 ||
+                  grad_stride < out_features;  // a row that stands for several (an expanded gradient)
+  p.padded = p.split_first ? (out_features + 7) / 8 * 8 : grad_stride;
+  p.parts_bytes = p.split_first ? (p.parts * rows * p.padded * 2 + 255) / 256 * 256 : 0;
+  p.steps_per_part = (uint32_t)((rows + kStep - 1) / kStep);
+  p.steps = p.steps_per_part * p.parts;
+  const int64_t large_tiles = ((out_features + 255) / 256) * ((features + 255) / 256);
+  p.large = large_tiles >= 128;
+  const int64_t size = p.large ? 256 : 128;
+  p.tiles_o = (uint32_t)((out_features + size - 1) / size);
+  p.tiles_f = (uint32_t)((features + size - 1) / size);
+  const int64_t tiles = (int64_t)p.tiles_o * p.tiles_f;
+  const int64_t wanted = p.large ? 256 : 512;
+  int64_t splits = tiles >= wanted ? 1 : wanted / tiles;
+  const int64_t most = p.steps / 4 > 1 ? p.steps / 4 : 1;
+  if (splits > most) splits = most;
+  p.splits = (uint32_t)splits;
+  p.partial_bytes = splits > 1 ? splits * out_features * pitch * 4 : 0;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tft_pack_e4m3(void* values, void* exponents, const void* x, int64_t rows, int64_t features,
+                  int64_t x_row_stride, int64_t pitch, int dtype, void* stream) {
+  static const char* what = "tft_pack_e4m3";
+  if (int rc = check_types(what, dtype, 0, false)) return rc;
+  if (rows < 0 || features < 0) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+  if (rows == 0 || features == 0) return TFT_OK;
+  if (int rc = check_packed(what, values, exponents, rows, features, pitch)) return rc;
+  if (!x || misaligned(x, dtype)) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: x is NULL or misaligned", what);
+  if (x_row_stride < 0) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: negative row stride", what);
+  const uint32_t per_row = (uint32_t)((features + kBlock - 1) / kBlock);
+  PackArgs a{x, static_cast<uint8_t*>(values), static_cast<uint8_t*>(exponents), features, x_row_stride,
+             pitch, (uint32_t)(rows * per_row), make_divider(per_row)};
+  void* params[] = {&a};
+  const dim3 grid((a.blocks + kPackBlocks - 1) / kPackBlocks);
+  const void* k = dtype == TFT_F32 ? TFT_KERNEL(pack_kernel<F32>)
+                  : dtype == TFT_BF16 ? TFT_KERNEL(pack_kernel<BF16>)
+                                      : TFT_KERNEL(pack_kernel<F16>);
+  return launch(what, k, grid, kPackThreads, params, static_cast<hipStream_t>(stream));
+}
+
+int tft_unpack_e4m3(void* out, const void* values, const void* exponents, const void* column_scale,
+                    int64_t rows, int64_t features, int64_t pitch, int scale_dtype, int dtype,
+                    void* stream) {
+  static const char* what = "tft_unpack_e4m3";
+  if (int rc = check_types(what, dtype, scale_dtype, column_scale != nullptr)) return rc;
+  if (rows < 0 || features < 0) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+  if (rows == 0 || features == 0) return TFT_OK;
+  if (int rc = check_packed(what, values, exponents, rows, features, pitch)) return rc;
+  if (!out || misaligned(out, dtype)) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: out is NULL or misaligned", what);
+  if (column_scale && misaligned(column_scale, scale_dtype))
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: column_scale is misaligned", what);
+  const uint32_t per_row = (uint32_t)((features + kBlock - 1) / kBlock);
+  UnpackArgs a{out, static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents), column_scale,
+               features, pitch, (uint32_t)(rows * per_row), make_divider(per_row)};
+  void* params[] = {&a};
+  const dim3 grid((a.blocks + kPackBlocks - 1) / kPackBlocks);
+  const int st = column_scale ? scale_dtype : TFT_F32;
+#define TFT_UNPACK(T)                                                     \
+  (st == TFT_F32 ? TFT_KERNEL(unpack_kernel<T, F32>)                      \
+   : st == TFT_BF16 ? TFT_KERNEL(unpack_kernel<T, BF16>)                  \
+                    : TFT_KERNEL(unpack_kernel<T, F16>))
+  const void* k = dtype == TFT_F32 ? TFT_UNPACK(F32) : dtype == TFT_BF16 ? TFT_UNPACK(BF16) : TFT_UNPACK(F16);
+#undef TFT_UNPACK
+  return launch(what, k, grid, kPackThreads, params, static_cast<hipStream_t>(stream));
+}
+
+int tft_rms_norm(void* y, void* h, void* values, void* exponents, float* rstd, const void* x,
+                 const void* residual, const void* weight, int64_t rows, int64_t features,
+                 int64_t x_row_stride, int64_t residual_row_stride, int64_t pitch, float eps,
+                 int weight_dtype, int dtype, void* stream) {
+  static const char* what = "tft_rms_norm";
+  if (int rc = check_types(what, dtype, weight_dtype, weight != nullptr)) return rc;
+  if (weight && weight_dtype != dtype && weight_dtype != TFT_F32)
+    return fail(TFT_ERR_UNSUPPORTED, "%s: the weight is of the activations' dtype or fp32", what);
+  if (rows < 0 || features < 0) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+  if (features > kMostNormFeatures)
+    return fail(TFT_ERR_UNSUPPORTED, "%s: %lld features, at most %d", what, (long long)features, kMostNormFeatures);
+  if (rows == 0 || features == 0) return TFT_OK;
+  if (rows >= kMostRows) return fail(TFT_ERR_UNSUPPORTED, "%s: %lld rows, at most 2^31 - 1", what, (long long)rows);
+  if (values || exponents)
+    if (int rc = check_packed(what, values, exponents, rows, features, pitch)) return rc;
+  if (!x || !y || misaligned(x, dtype) || misaligned(y, dtype))
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: x or y is NULL or misaligned", what);
+  if ((residual != nullptr) != (h != nullptr))
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: residual and h come together", what);
+  if (residual && (misaligned(residual, dtype) || misaligned(h, dtype)))
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: residual or h is misaligned", what);
+  if (weight && misaligned(weight, weight_dtype))
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: weight is misaligned", what);
+  if (x_row_stride < 0 || residual_row_stride < 0)
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: negative row stride", what);
+  if (!(eps >= 0.0f)) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: eps must be at least 0", what);
+  NormArgs a{x, residual, weight, y, h, static_cast<uint8_t*>(values), static_cast<uint8_t*>(exponents), rstd,
+             (uint32_t)rows, (int)features, x_row_stride, residual_row_stride, pitch,
+             weight_dtype == TFT_F32 ? 1 : 0, eps};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == TFT_F32) return launch_norm<F32>(what, a, s);
+  if (dtype == TFT_BF16) return launch_norm<BF16>(what, a, s);
+  return launch_norm<F16>(what, a, s);
+}
+
+int64_t tft_rms_norm_backward_workspace(int64_t rows, int64_t features) {
+  if (rows <= 0 || features <= 0 || rows >= kMostRows || features > kMostNormFeatures) return 0;
+  return (int64_t)norm_back_groups(rows, features) * features * 4;
+}
+
+int tft_rms_norm_backward(void* grad_x, void* grad_weight, void* workspace, int64_t workspace_bytes,
+                          const void* grad_y, const void* grad_h, const void* values,
+                          const void* exponents, const float* rstd, const void* weight, int64_t rows,
+                          int64_t features, int64_t grad_y_row_stride, int64_t grad_h_row_stride,
+                          int64_t pitch, int weight_dtype, int dtype, void* stream) {
+  static const char* what = "tft_rms_norm_backward";
+  if (int rc = check_types(what, dtype, weight_dtype, weight != nullptr || grad_weight != nullptr)) return rc;
+  if ((weight || grad_weight) && weight_dtype != dtype && weight_dtype != TFT_F32)
+    return fail(TFT_ERR_UNSUPPORTED, "%s: the weight is of the activations' dtype or fp32", what);
+  if (rows < 0 || features < 0) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+  if (features > kMostNormFeatures)
+    return fail(TFT_ERR_UNSUPPORTED, "%s: %lld features, at most %d", what, (long long)features, kMostNormFeatures);
+  if (features == 0) return TFT_OK;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (grad_weight && misaligned(grad_weight, weight_dtype))
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: grad_weight is misaligned", what);
+  if (rows == 0)  // the empty sum
+    return grad_weight ? launch_column_reduce(what, nullptr, grad_weight, 0, features, weight_dtype, s) : TFT_OK;
+  if (int rc = check_packed(what, values, exponents, rows, features, pitch)) return rc;
+  if (!grad_x || !grad_y || !rstd || misaligned(grad_x, dtype) || misaligned(grad_y, dtype) ||
+      misaligned(rstd, TFT_F32))
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: grad_x, grad_y or rstd is NULL or misaligned", what);
+  if (grad_h && misaligned(grad_h, dtype)) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: grad_h is misaligned", what);
+  if (weight && misaligned(weight, weight_dtype))
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: weight is misaligned", what);
+  if (grad_y_row_stride < 0 || grad_h_row_stride < 0)
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: negative row stride", what);
+  if (grad_weight && (!workspace || misaligned(workspace, TFT_F32) ||
+                      workspace_bytes < tft_rms_norm_backward_workspace(rows, features)))
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: workspace of %lld bytes, %lld are needed", what,
+                (long long)workspace_bytes, (long long)tft_rms_norm_backward_workspace(rows, features));
+  float* partial = grad_weight ? static_cast<float*>(workspace) : nullptr;
+  NormBackArgs a{grad_y, grad_h, static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents), rstd,
+                 weight, grad_x, partial, (uint32_t)rows, (int)features, grad_y_row_stride, grad_h_row_stride,
+                 pitch, weight_dtype == TFT_F32 ? 1 : 0};
+  int rc;
+  if (dtype == TFT_F32) rc = launch_norm_back<F32>(what, a, s);
+  else if (dtype == TFT_BF16) rc = launch_norm_back<BF16>(what, a, s);
+  else rc = launch_norm_back<F16>(what, a, s);
+  if (rc || !grad_weight) return rc;
+  return launch_column_reduce(what, partial, grad_weight, norm_back_groups(rows, features), features,
+                              weight_dtype, s);
+}
+
+int64_t tft_column_sum_workspace(int64_t rows, int64_t columns) {
+  if (rows <= 0 || columns <= 0 || rows >= kMostRows || columns >= kMostRows) return 0;
+  return (int64_t)column_sum_groups(rows, columns) * columns * 4;
+}
+
+int tft_column_sum(void* out, void* workspace, int64_t workspace_bytes, const void* x, int64_t rows,
+                   int64_t columns, int64_t x_row_stride, int out_dtype, int dtype, void* stream) {
+  static const char* what = "tft_column_sum";
+  if (int rc = check_types(what, dtype, out_dtype, true)) return rc;
+  if (rows < 0 || columns < 0) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+  if (columns == 0) return TFT_OK;
+  if (rows >= kMostRows || columns >= kMostRows)
+    return fail(TFT_ERR_UNSUPPORTED, "%s: at most 2^31 - 1 rows and columns", what);
+  if (!out || misaligned(out, out_dtype)) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: out is NULL or misaligned", what);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (rows == 0) return launch_column_reduce(what, nullptr, out, 0, columns, out_dtype, s);
+  if (!x || misaligned(x, dtype)) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: x is NULL or misaligned", what);
+  if (x_row_stride < 0) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: negative row stride", what);
+  if (!workspace || misaligned(workspace, TFT_F32) || workspace_bytes < tft_column_sum_workspace(rows, columns))
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: workspace of %lld bytes, %lld are needed", what,
+                (long long)workspace_bytes, (long long)tft_column_sum_workspace(rows, columns));
+  float* partial = static_cast<float*>(workspace);
+  uint32_t r = (uint32_t)rows;
+  void* params[] = {&x, &partial, &r, &columns, &x_row_stride};
+  const dim3 grid((uint32_t)((columns + 2047) / 2048), column_sum_groups(rows, columns));
+  const void* k = dtype == TFT_F32 ? TFT_KERNEL(column_sum_kernel<F32>)
+                  : dtype == TFT_BF16 ? TFT_KERNEL(column_sum_kernel<BF16>)
+                                      : TFT_KERNEL(column_sum_kernel<F16>);
+  if (int rc = launch(what, k, grid, 256, params, s)) return rc;
+  return launch_column_reduce(what, partial, out, grid.y, columns, out_dtype, s);
+}
+
+int64_t tft_linear_weight_grad_workspace(const void* grad_out, int64_t rows, int64_t out_features,
+                                         int64_t features, int64_t grad_row_stride, int64_t pitch,
+                                         int dtype) {
+  if (rows <= 0 || out_features <= 0 || features <= 0) return 0;
+  const WgradPlan p = plan_wgrad(rows, out_features, features, pitch, grad_row_stride, dtype,
+                                 (reinterpret_cast<uintptr_t>(grad_out) & 15u) == 0);
+  return p.parts_bytes + p.partial_bytes;
+}
+
+int tft_linear_weight_grad(void* grad_weight, void* workspace, int64_t workspace_bytes,
+                           const void* grad_out, const void* values, const void* exponents,
+                           const void* column_scale, int64_t rows, int64_t out_features,
+                           int64_t features, int64_t grad_row_stride, int64_t pitch, int out_dtype,
+                           int scale_dtype, int dtype, void* stream) {
+  static const char* what = "tft_linear_weight_grad";
+  if (int rc = check_types(what, dtype, scale_dtype, column_scale != nullptr)) return rc;
+  if (int rc = check_types(what, out_dtype, 0, false)) return rc;
+  if (rows < 0 || out_features < 0 || features < 0)
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+  if (out_features == 0 || features == 0) return TFT_OK;
+  if (out_features >= kMostRows) return fail(TFT_ERR_UNSUPPORTED, "%s: at most 2^31 - 1 output features", what);
+  if (!grad_weight || (reinterpret_cast<uintptr_t>(grad_weight) & 15u))
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: grad_weight is NULL or not at a multiple of 16 bytes", what);
+  if (rows > 0) {
+    if (int rc = check_packed(what, values, exponents, rows, features, pitch)) return rc;
+    if (!grad_out || misaligned(grad_out, dtype))
+      return fail(TFT_ERR_INVALID_ARGUMENT, "%s: grad_out is NULL or misaligned", what);
+    if (grad_row_stride < 0) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: negative row stride", what);
+  }
+  if (column_scale && misaligned(column_scale, scale_dtype))
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: column_scale is misaligned", what);
+  const WgradPlan p = plan_wgrad(rows, out_features, features, pitch, grad_row_stride, dtype,
+                                 (reinterpret_cast<uintptr_t>(grad_out) & 15u) == 0);
+  // offsets within a step's rows are 31 bits
+  if (p.padded * 2 * kStep >= (1ll << 31) || pitch * kStep >= (1ll << 31))
+    return fail(TFT_ERR_UNSUPPORTED, "%s: rows of %lld gradients or %lld packed values are too long", what,
+                (long long)p.padded, (long long)pitch);
+  if ((int64_t)p.steps_per_part * p.parts >= (1ll << 31) ||
+      (int64_t)p.tiles_o * p.tiles_f * p.splits >= (1ll << 31))
+    return fail(TFT_ERR_UNSUPPORTED, "%s: too many tiles for one grid", what);
+  const int64_t needed = p.parts_bytes + p.partial_bytes;
+  if (needed && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < needed))
+    return fail(TFT_ERR_INVALID_ARGUMENT, "%s: workspace of %lld bytes, %lld are needed", what,
+                (long long)workspace_bytes, (long long)needed);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const uint16_t* d = static_cast<const uint16_t*>(grad_out);
+  if (p.split_first && rows > 0) {
+    SplitArgs a{grad_out, static_cast<uint16_t*>(workspace), rows, out_features, grad_row_stride, p.padded,
+                (uint64_t)rows * (p.padded / 8)};
+    void* params[] = {&a};
+    const uint64_t groups = (a.chunks + 255) / 256;
+    const dim3 grid((uint32_t)(groups < 16384 ? groups : 16384));
+    const void* k = dtype == TFT_F32 ? TFT_KERNEL(split_kernel<F32, 3>)
+                    : dtype == TFT_BF16 ? TFT_KERNEL(split_kernel<BF16, 1>)
+                                        : TFT_KERNEL(split_kernel<F16, 2>);
+    if (int rc = launch(what, k, grid, 256, params, s)) return rc;
+    d = a.parts;
+  }
+  float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.parts_bytes);
+  WgradArgs a{d, static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents), column_scale,
+              p.splits > 1 ? static_cast<void*>(partial) : grad_weight, rows, p.padded, pitch,
+              (uint32_t)out_features, (uint32_t)features, (uint32_t)((features + kBlock - 1) / kBlock),
+              p.tiles_o, p.tiles_f, p.splits, p.steps_per_part, p.steps, scale_dtype, out_dtype,
+              p.splits > 1 ? 1 : 0};
+  void* params[] = {&a};
+  const dim3 grid(p.tiles_o * p.tiles_f * p.splits);
+  if (int rc = p.large ? launch(what, TFT_KERNEL(wgrad_kernel<256, 256, 2, 4>), grid, 512, params, s)
+                       : launch(what, TFT_KERNEL(wgrad_kernel<128, 128, 2, 2>), grid, 256, params, s))
+    return rc;
+  if (p.splits == 1) return TFT_OK;
+  a.out = grad_weight;
+  const float* from = partial;
+  void* join_params[] = {&a, &from};
+  const uint64_t groups = ((uint64_t)out_features * (pitch / 4) + 255) / 256;
+  return launch(what, TFT_KERNEL(wgrad_join_kernel), dim3((uint32_t)(groups < 16384 ? groups : 16384)), 256,
+                join_params, s);
+}
+
+}  // extern "C"

@@ -25,27 +25,35 @@
 
 #include <mutex>
 
+#include "errors.h"
 #include "torchft_amd.h"
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxCols = TFT_MAX_REPLICAS + 3;
-
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 thread_local char g_err[512] = "";
-#ifdef TFT_TUNING
-thread_local uint32_t g_variant = 0;  // tuning builds only: overrides the launch shape
-#endif
 
-int fail(int code, const char* fmt, ...) {
+}  // namespace
+
+int tft::fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof(g_err), fmt, ap);
   va_end(ap);
   return code;
 }
+
+namespace {
+
+using tft::fail;
+
+constexpr int kThreads = 256;
+constexpr int kMaxCols = TFT_MAX_REPLICAS + 3;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+#ifdef TFT_TUNING
+thread_local uint32_t g_variant = 0;  // tuning builds only: overrides the launch shape
+#endif
 
 // ---------------------------------------------------------------------------
 // Element types: how a 16-byte vector is widened to fp32 lanes and back.

@@ -24,6 +24,7 @@ from torch import nn
 from torch.nn import parallel
 
 from . import ops
+from .activations import pack_activations
 from .multi_tensor import TensorTable
 from .process_group import ProcessGroupDummy
 
@@ -39,10 +40,17 @@ class DistributedDataParallel(parallel.DistributedDataParallel):
     (torchft/ddp.py:32-71).  A dummy process group absorbs the constructor's
     collectives; ``find_unused_parameters=True`` stops the Reducer from rebuilding
     its buckets after the first step, which would make a recovering replica's bucket
-    layout differ from its peers'."""
+    layout differ from its peers'.
 
-    def __init__(self, manager: "Manager", module: nn.Module, **kwargs: object) -> None:
+    ``packed_activations=True`` makes the ``nn.Linear`` and ``nn.RMSNorm`` modules of ``module``
+    keep their activations in 8 bits for the backward pass (``activations.pack_activations``)."""
+
+    def __init__(
+        self, manager: "Manager", module: nn.Module, *, packed_activations: bool = False, **kwargs: object
+    ) -> None:
         pg = ProcessGroupDummy(0, 1)
+        if packed_activations:
+            pack_activations(module)
         super().__init__(
             module,
             process_group=pg,
@@ -60,11 +68,12 @@ class DistributedDataParallel(parallel.DistributedDataParallel):
 
 class PureDistributedDataParallel(nn.Module):
     """DDP without a Reducer: one ``manager.allreduce`` per gradient as soon as it has
-    been accumulated (torchft/ddp.py:74-97)."""
+    been accumulated (torchft/ddp.py:74-97).  ``packed_activations`` as for
+    :class:`DistributedDataParallel`."""
 
-    def __init__(self, manager: "Manager", module: nn.Module) -> None:
+    def __init__(self, manager: "Manager", module: nn.Module, *, packed_activations: bool = False) -> None:
         super().__init__()
-        self.module = module
+        self.module = pack_activations(module) if packed_activations else module
 
         def post_grad_hook(p: torch.Tensor) -> None:
             if p.grad is not None:
