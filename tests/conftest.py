@@ -22,6 +22,12 @@ def pytest_collection_modifyitems(config, items):
             item.add_marker(skip)
 
 
+@pytest.fixture(autouse=True)
+def seeded():
+    """Weights that a test does not seed itself are the same in every run."""
+    torch.manual_seed(0)
+
+
 @pytest.fixture(scope="session")
 def device():
     return torch.device("cuda", 0)
