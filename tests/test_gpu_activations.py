@@ -492,7 +492,8 @@ def test_captured_steps_replay(device):
             out = model(x)
             gr = torch.autograd.grad((out * target).sum(), params)
         graphs.append(g)
-        outs.append(out)
+        outs.append(out.detach())
+        del out  # no autograd graph of these leaves outlives its capture
         grads.append(gr)
     for k in range(4):
         x.copy_(randn(k, 130, 192, dtype=torch.bfloat16))

@@ -28,7 +28,6 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import _native
-from .multi_tensor import current_stream_handle
 
 BLOCK = 128  # features that share a scale
 MAX_NORM_FEATURES = 16384
@@ -45,6 +44,25 @@ def _dtype_code(dtype: torch.dtype, what: str) -> int:
         return _DTYPES[dtype]
     except KeyError:
         raise TypeError(f"{what}: float32, bfloat16 and float16 are supported, got {dtype}") from None
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _launch(name: str, device: torch.device, *args: object) -> None:
+    """One C entry on the device's current stream.  The smallest calls are a few microseconds of
+    GPU time, so the device is only switched where it is not the current one, and the stream is
+    asked for without an object around it (1.2 and 1.8 microseconds of 10)."""
+    index = device.index
+    fn = getattr(_native.lib(), name)
+    if _current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _native.check(rc, name)
 
 
 def _require_gpu(t: torch.Tensor, what: str) -> None:
@@ -191,14 +209,11 @@ class PackedActivation:
         device = self.values.device
         out = torch.empty(self.shape, dtype=dtype, device=device)
         scale = self.column_scale
-        with torch.cuda.device(device):
-            rc = _native.lib().tft_unpack_e4m3(
-                out.data_ptr(), self.values.data_ptr(), self.exponents.data_ptr(),
-                None if scale is None else scale.data_ptr(), self.rows, self.features,
-                self.values.shape[1], code if scale is None else _DTYPES[scale.dtype], code,
-                current_stream_handle(device),
-            )
-        _native.check(rc, "tft_unpack_e4m3")
+        _launch(
+            "tft_unpack_e4m3", device, out.data_ptr(), self.values.data_ptr(), self.exponents.data_ptr(),
+            None if scale is None else scale.data_ptr(), self.rows, self.features,
+            self.values.shape[1], code if scale is None else _DTYPES[scale.dtype], code,
+        )
         return out
 
 
@@ -224,12 +239,10 @@ def pack(x: torch.Tensor) -> PackedActivation:
     code = _dtype_code(x.dtype, "pack")
     device = x.device
     values, exponents = _buffers(rows, features, device)
-    with torch.cuda.device(device):
-        rc = _native.lib().tft_pack_e4m3(
-            values.data_ptr(), exponents.data_ptr(), x.data_ptr(), rows, features, stride,
-            values.shape[1], code, current_stream_handle(device),
-        )
-    _native.check(rc, "tft_pack_e4m3")
+    _launch(
+        "tft_pack_e4m3", device, values.data_ptr(), exponents.data_ptr(), x.data_ptr(), rows, features,
+        stride, values.shape[1], code,
+    )
     return _trusted(values, exponents, features, None, tuple(x.shape), x.dtype)
 
 
@@ -275,16 +288,13 @@ def rms_norm_forward(
     if pack:
         values, exponents = _buffers(rows, features, device)
         packed = _trusted(values, exponents, features, weight, tuple(x.shape), x.dtype)
-    with torch.cuda.device(device):
-        rc = _native.lib().tft_rms_norm(
-            y.data_ptr(), None if residual is None else h.data_ptr(),
-            values.data_ptr() if pack else None, exponents.data_ptr() if pack else None,
-            rstd.data_ptr(), x.data_ptr(), None if residual is None else residual.data_ptr(),
-            None if weight is None else weight.data_ptr(), rows, features, stride, residual_stride,
-            values.shape[1] if pack else 0, eps, code if weight is None else _DTYPES[weight.dtype],
-            code, current_stream_handle(device),
-        )
-    _native.check(rc, "tft_rms_norm")
+    _launch(
+        "tft_rms_norm", device, y.data_ptr(), None if residual is None else h.data_ptr(),
+        values.data_ptr() if pack else None, exponents.data_ptr() if pack else None,
+        rstd.data_ptr(), x.data_ptr(), None if residual is None else residual.data_ptr(),
+        None if weight is None else weight.data_ptr(), rows, features, stride, residual_stride,
+        values.shape[1] if pack else 0, eps, code if weight is None else _DTYPES[weight.dtype], code,
+    )
     return y, h, packed, rstd
 
 
@@ -327,17 +337,15 @@ def rms_norm_backward(
         grad_weight = torch.empty(features, dtype=weight.dtype, device=device)
         need = _native.lib().tft_rms_norm_backward_workspace(rows, features)
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    with torch.cuda.device(device):
-        rc = _native.lib().tft_rms_norm_backward(
-            grad_x.data_ptr(), None if grad_weight is None else grad_weight.data_ptr(),
-            None if workspace is None else workspace.data_ptr(), need, grad_y.data_ptr(),
-            None if grad_h is None else grad_h.data_ptr(), packed.values.data_ptr(),
-            packed.exponents.data_ptr(), rstd.data_ptr(),
-            None if weight is None else weight.data_ptr(), rows, features, stride, grad_h_stride,
-            packed.values.shape[1], code if weight is None else _DTYPES[weight.dtype], code,
-            current_stream_handle(device),
-        )
-    _native.check(rc, "tft_rms_norm_backward")
+    _launch(
+        "tft_rms_norm_backward", device, grad_x.data_ptr(),
+        None if grad_weight is None else grad_weight.data_ptr(),
+        None if workspace is None else workspace.data_ptr(), need, grad_y.data_ptr(),
+        None if grad_h is None else grad_h.data_ptr(), packed.values.data_ptr(),
+        packed.exponents.data_ptr(), rstd.data_ptr(),
+        None if weight is None else weight.data_ptr(), rows, features, stride, grad_h_stride,
+        packed.values.shape[1], code if weight is None else _DTYPES[weight.dtype], code,
+    )
     return grad_x, grad_weight
 
 
@@ -359,20 +367,17 @@ def linear_weight_grad(
     scale = packed.column_scale
     features, pitch = packed.features, packed.values.shape[1]
     out = torch.empty(out_features, features, dtype=dtype, device=device)
-    lib = _native.lib()
-    need = lib.tft_linear_weight_grad_workspace(
+    need = _native.lib().tft_linear_weight_grad_workspace(
         grad_out.data_ptr(), rows, out_features, features, stride, pitch, code
     )
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    with torch.cuda.device(device):
-        rc = lib.tft_linear_weight_grad(
-            out.data_ptr(), None if workspace is None else workspace.data_ptr(), need,
-            grad_out.data_ptr(), packed.values.data_ptr(), packed.exponents.data_ptr(),
-            None if scale is None else scale.data_ptr(), rows, out_features, features, stride, pitch,
-            out_code, code if scale is None else _DTYPES[scale.dtype], code,
-            current_stream_handle(device),
-        )
-    _native.check(rc, "tft_linear_weight_grad")
+    _launch(
+        "tft_linear_weight_grad", device, out.data_ptr(),
+        None if workspace is None else workspace.data_ptr(), need, grad_out.data_ptr(),
+        packed.values.data_ptr(), packed.exponents.data_ptr(),
+        None if scale is None else scale.data_ptr(), rows, out_features, features, stride, pitch,
+        out_code, code if scale is None else _DTYPES[scale.dtype], code,
+    )
     return out
 
 
@@ -384,15 +389,12 @@ def column_sum(x: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Te
     code = _dtype_code(x.dtype, what)
     dtype = x.dtype if dtype is None else dtype
     out = torch.empty(columns, dtype=dtype, device=x.device)
-    lib = _native.lib()
-    need = lib.tft_column_sum_workspace(rows, columns)
+    need = _native.lib().tft_column_sum_workspace(rows, columns)
     workspace = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    with torch.cuda.device(x.device):
-        rc = lib.tft_column_sum(
-            out.data_ptr(), None if workspace is None else workspace.data_ptr(), need, x.data_ptr(),
-            rows, columns, stride, _dtype_code(dtype, what), code, current_stream_handle(x.device),
-        )
-    _native.check(rc, "tft_column_sum")
+    _launch(
+        "tft_column_sum", x.device, out.data_ptr(), None if workspace is None else workspace.data_ptr(),
+        need, x.data_ptr(), rows, columns, stride, _dtype_code(dtype, what), code,
+    )
     return out
 
 

@@ -34,6 +34,7 @@ typedef u32x4 u32x4_a2 __attribute__((aligned(2)));  // rows start where they st
 typedef u32x4 u32x4_a4 __attribute__((aligned(4)));  // 128 bits from any address
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -712,14 +713,30 @@ struct WgradArgs {
   const uint8_t* values;
   const uint8_t* exponents;
   const void* column_scale;  // or NULL
-  void* out;                 // [out_features][features], or fp32 [splits][out_features][pitch]
+  void* out;                 // [out_features][features]
+  float* partial;            // [splits][cut tiles][tile], or NULL
   int64_t rows, d_stride, pitch;
   uint32_t out_features, features, blocks;
-  uint32_t tiles_o, tiles_f, splits;
+  uint32_t tiles_o, tiles_f;
+  uint32_t whole, cut, splits;     // tiles of one workgroup each, tiles of `splits` workgroups each
   uint32_t steps_per_part, steps;  // of all parts
   int scale_type, out_type;        // TFT_F32 ...
-  int to_partial;
 };
+
+// Workgroup ids go round the 8 XCDs in turn; this gives each of them a run of neighbouring
+// numbers out of n, so that what its workgroups share stays in its own L2.
+__device__ inline uint32_t neighbours_on_an_xcd(uint32_t id, uint32_t n) {
+  const uint32_t xcd = id % 8, each = n / 8, more = n % 8;
+  return xcd * each + min(xcd, more) + id / 8;
+}
+
+// Tiles are numbered down bands of four rows of tiles: 32 in a row, one XCD's worth, are 4 x 8.
+__device__ inline void tile_at(const WgradArgs& a, uint32_t n, uint32_t* o, uint32_t* f) {
+  const uint32_t band = n / (4 * a.tiles_f), in_band = n - band * 4 * a.tiles_f;
+  const uint32_t high = min(4u, a.tiles_o - band * 4);
+  *o = band * 4 + in_band % high;
+  *f = in_band / high;
+}
 
 __device__ inline __amdgpu_buffer_rsrc_t buffer(const void* base, int64_t bytes) {
   // reads behind the end give zero
@@ -771,26 +788,34 @@ __device__ inline void store_out4(const WgradArgs& a, int64_t o, int64_t f, f32x
 // Both operands lie with the summed axis (tokens) outermost, so LDS holds a step's tiles as they
 // lie in memory, [token][column], and the transposing LDS reads (ds_read_b64_tr_b16: 16 lanes
 // fetch 4 tokens x 16 columns, lane i gets column i's four tokens) turn them into matrix
-// operands.  A lane's eight tokens of a 32-token product are 4g + 0..3 and 16 + 4g + 0..3 for
-// lane group g, the same in both operands.  Rows of a tile are 16-column units of 32 bytes; unit
-// u of token t lies at u ^ (t & 7), which spreads the four rows of a transposing read, and the
-// rows of two neighbouring lane groups, over all banks.
+// operands: lanes 0 .. 31 hold a product's first eight tokens of 32 columns, lanes 32 .. 63 the
+// other eight.  Rows of a tile are units of 16 columns (32 bytes); unit u of token t lies at
+// u ^ spread(t), so that the four rows of a transposing read, and the two units that lanes 0 .. 31
+// read together, lie on different banks.
+__device__ inline int spread(int t) { return (t & 3) | ((t & 1) << 2); }
+
 template <int O, int F, int WO, int WF>
-__global__ __launch_bounds__(64 * WO * WF) void wgrad_kernel(WgradArgs a) {
+__global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
   constexpr int kThreads = 64 * WO * WF;
   constexpr int kDChunks = kStep * O / 8 / kThreads;   // 16-byte chunks of D per thread and step
   constexpr int kXChunks = kStep * F / 16 / kThreads;  // 16-byte chunks of X
-  constexpr int kFragO = O / WO / 16, kFragF = F / WF / 16;
-  __shared__ __attribute__((aligned(128))) uint16_t lds_d[2][kStep * O];
-  __shared__ __attribute__((aligned(128))) uint16_t lds_x[2][kStep * F];
+  constexpr int kFragO = O / WO / 32, kFragF = F / WF / 32;
+  __shared__ __attribute__((aligned(128))) uint16_t lds[2 * kStep * (O + F)];
+  uint16_t* const lds_d = lds;                  // two tiles of kStep x O
+  uint16_t* const lds_x = lds + 2 * kStep * O;  // two tiles of kStep x F
 
-  const uint32_t tiles = a.tiles_o * a.tiles_f;
-  const uint32_t split = blockIdx.x / tiles;
-  const uint32_t tile = blockIdx.x - split * tiles;
-  const int64_t o0 = (int64_t)(tile / a.tiles_f) * O;
-  const int64_t f0 = (int64_t)(tile % a.tiles_f) * F;
-  const uint32_t step_begin = (uint32_t)((uint64_t)a.steps * split / a.splits);
-  const uint32_t step_end = (uint32_t)((uint64_t)a.steps * (split + 1) / a.splits);
+  const bool is_cut = blockIdx.x >= a.whole;
+  uint32_t tile_o, tile_f, slot = 0, step_begin = 0, step_end = a.steps;
+  if (is_cut) {
+    slot = neighbours_on_an_xcd(blockIdx.x - a.whole, a.cut * a.splits);  // split-major
+    const uint32_t split = slot / a.cut;
+    step_begin = (uint32_t)((uint64_t)a.steps * split / a.splits);
+    step_end = (uint32_t)((uint64_t)a.steps * (split + 1) / a.splits);
+    tile_at(a, a.whole + slot - split * a.cut, &tile_o, &tile_f);
+  } else {
+    tile_at(a, neighbours_on_an_xcd(blockIdx.x, a.whole), &tile_o, &tile_f);
+  }
+  const int64_t o0 = (int64_t)tile_o * O, f0 = (int64_t)tile_f * F;
 
   // what this thread stages, the same in every step but for the token offset
   uint32_t d_off[kDChunks], d_lds[kDChunks], x_off[kXChunks], x_lds[kXChunks], e_off[kXChunks];
@@ -798,142 +823,218 @@ __global__ __launch_bounds__(64 * WO * WF) void wgrad_kernel(WgradArgs a) {
   for (int i = 0; i < kDChunks; ++i) {
     const int c = i * kThreads + threadIdx.x, t = c / (O / 8), j = c % (O / 8);
     d_off[i] = o0 + j * 8 < a.out_features ? (uint32_t)((t * a.d_stride + j * 8) * 2) : 0x80000000u;
-    d_lds[i] = t * O + (((j >> 1) ^ (t & 7)) << 4) + ((j & 1) << 3);
+    d_lds[i] = t * O + (((j >> 1) ^ spread(t)) << 4) + ((j & 1) << 3);
   }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int swap = (lane >> 2) & 1;  // lanes 4 .. 7 of eight write a unit's halves the other way round
 #pragma unroll
   for (int i = 0; i < kXChunks; ++i) {
     const int c = i * kThreads + threadIdx.x, t = c / (F / 16), u = c % (F / 16);
     x_off[i] = f0 + u * 16 < a.pitch ? (uint32_t)(t * a.pitch + u * 16) : 0x80000000u;
     e_off[i] = f0 + u * 16 < a.pitch ? (uint32_t)(t * a.blocks + (u * 16) / kBlock) : 0x80000000u;
-    x_lds[i] = t * F + ((u ^ (t & 7)) << 4);
+    x_lds[i] = t * F + ((u ^ spread(t)) << 4) + swap * 8;
   }
-  // what this lane reads: token 4g + i / 4 (+ 16, + 32 ...), columns 4 (i % 4) .. of unit u
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int t_lane = ((lane >> 4) << 2) + ((lane & 15) >> 2);
+  // what this lane reads: token 8 (lane / 32) + i / 4 of a product's 16 (+ 4), columns 4 (i % 4) ..
+  // of unit 2f + (lane / 16) % 2, for lane i of 16
+  const int t_lane = ((lane >> 5) << 3) + ((lane & 15) >> 2);
   const int wave_o = (wave / WF) * (O / WO), wave_f = (wave % WF) * (F / WF);
   uint32_t d_read[kFragO], x_read[kFragF];
 #pragma unroll
   for (int f = 0; f < kFragO; ++f)
-    d_read[f] = t_lane * O + (((wave_o / 16 + f) ^ (t_lane & 7)) << 4) + ((lane & 3) << 2);
+    d_read[f] = t_lane * O + (((wave_o / 16 + 2 * f + ((lane >> 4) & 1)) ^ spread(t_lane)) << 4) + ((lane & 3) << 2);
 #pragma unroll
   for (int f = 0; f < kFragF; ++f)
-    x_read[f] = t_lane * F + (((wave_f / 16 + f) ^ (t_lane & 7)) << 4) + ((lane & 3) << 2);
+    x_read[f] = t_lane * F + (((wave_f / 16 + 2 * f + ((lane >> 4) & 1)) ^ spread(t_lane)) << 4) + ((lane & 3) << 2);
 
+  // the staged tile of one step: d, x and e point at its first token and column
+  const uint16_t* d_at;
+  const uint8_t *x_at, *e_at;
+  int64_t left;  // tokens from there on
+  {
+    const uint32_t part = step_begin / a.steps_per_part;
+    const int64_t t0 = (int64_t)(step_begin - part * a.steps_per_part) * kStep;
+    d_at = a.d + ((int64_t)part * a.rows + t0) * a.d_stride + o0;
+    x_at = a.values + t0 * a.pitch + f0;
+    e_at = a.exponents + t0 * a.blocks + f0 / kBlock;
+    left = a.rows - t0;
+  }
+  uint32_t to_fetch = step_end - step_begin;
   u32x4 d_reg[kDChunks], x_reg[kXChunks];
   uint32_t e_reg[kXChunks];
-  auto fetch = [&](uint32_t step) {
-    const uint32_t part = step / a.steps_per_part;
-    const int64_t t0 = (int64_t)(step - part * a.steps_per_part) * kStep;
-    const int64_t left = a.rows - t0;
-    const auto d = buffer(a.d + ((int64_t)part * a.rows + t0) * a.d_stride + o0,
-                          (left * a.d_stride - o0) * 2);
-    const auto x = buffer(a.values + t0 * a.pitch + f0, left * a.pitch - f0);
-    const auto e = buffer(a.exponents + t0 * a.blocks + f0 / kBlock, left * a.blocks - f0 / kBlock);
+  // D and X are asked for at different times, each as soon as its registers are free
+  auto fetch_d = [&]() {
+    const int64_t rows = to_fetch ? left : 0;  // nothing is read behind the last step
+    const auto d = buffer(d_at, (rows * a.d_stride - o0) * 2);
 #pragma unroll
     for (int i = 0; i < kDChunks; ++i)
       d_reg[i] = __builtin_amdgcn_raw_buffer_load_b128(d, d_off[i], 0, 0);
+  };
+  auto fetch_x = [&]() {
+    const int64_t rows = to_fetch ? left : 0;
+    const auto x = buffer(x_at, rows * a.pitch - f0);
+    const auto e = buffer(e_at, rows * a.blocks - f0 / kBlock);
 #pragma unroll
     for (int i = 0; i < kXChunks; ++i) {
       x_reg[i] = __builtin_amdgcn_raw_buffer_load_b128(x, x_off[i], 0, 0);
       e_reg[i] = __builtin_amdgcn_raw_buffer_load_b8(e, e_off[i], 0, 0);
     }
   };
-  auto stage = [&](int buf) {
+  auto advance = [&]() {
+    to_fetch -= to_fetch ? 1 : 0;
+    left -= kStep;
+    d_at += kStep * a.d_stride;
+    x_at += kStep * a.pitch;
+    e_at += (int64_t)kStep * a.blocks;
+    if (left <= 0) {  // the next part starts behind this one's last row, X over again
+      d_at += left * a.d_stride;
+      x_at += (left - a.rows) * a.pitch;
+      e_at += (left - a.rows) * a.blocks;
+      left = a.rows;
+    }
+  };
+  auto stage_d = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < kDChunks; ++i)
-      *reinterpret_cast<u32x4*>(&lds_d[buf][d_lds[i]]) = d_reg[i];
-    const int swap = (lane >> 2) & 1;  // lanes 4 .. 7 of eight write their halves the other way round
+      *reinterpret_cast<u32x4*>(&lds_d[buf * kStep * O + d_lds[i]]) = d_reg[i];
+  };
+  auto stage_x = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < kXChunks; ++i) {
       const float scale = scale_of(e_reg[i]);
       u32x4 half[2];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        half[w >> 1][(w & 1) * 2] = __builtin_bit_cast(
-            uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x_reg[i][w], scale, false));
-        half[w >> 1][(w & 1) * 2 + 1] = __builtin_bit_cast(
-            uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x_reg[i][w], scale, true));
-      }
-      *reinterpret_cast<u32x4*>(&lds_x[buf][x_lds[i] + swap * 8]) = swap ? half[1] : half[0];
-      *reinterpret_cast<u32x4*>(&lds_x[buf][x_lds[i] + 8 - swap * 8]) = swap ? half[0] : half[1];
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint32_t from = (h ^ swap) ? x_reg[i][2 + w] : x_reg[i][w];
+          half[h][2 * w] = __builtin_bit_cast(
+              uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(from, scale, false));
+          half[h][2 * w + 1] = __builtin_bit_cast(
+              uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(from, scale, true));
+        }
+      *reinterpret_cast<u32x4*>(&lds_x[buf * kStep * F + x_lds[i]]) = half[0];
+      *reinterpret_cast<u32x4*>(&lds_x[buf * kStep * F + (x_lds[i] ^ 8)]) = half[1];
     }
   };
 
-  f32x4 acc[kFragF][kFragO];
+  f32x16 acc[kFragF][kFragO];
 #pragma unroll
   for (int i = 0; i < kFragF; ++i)
 #pragma unroll
-    for (int j = 0; j < kFragO; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < kFragO; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
   typedef __attribute__((address_space(3))) s16x4* lds_ptr;
   auto read_tr = [&](const uint16_t* p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(const_cast<uint16_t*>(p)));
   };
-  auto operand = [&](const uint16_t* base, int columns) {  // 32 tokens of one unit
-    const s16x4 lo = read_tr(base), hi = read_tr(base + 16 * columns);
+  auto operand = [&](const uint16_t* base, int columns) {  // 16 tokens of two units
+    const s16x4 lo = read_tr(base), hi = read_tr(base + 4 * columns);
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  auto multiply = [&](int buf) {
+  struct Operands {
+    bf16x8 d[kFragO], x[kFragF];
+  };
+  auto load = [&](Operands& to, int buf, int sub) {  // tokens 16 sub .. + 15
 #pragma unroll
-    for (int k = 0; k < kStep / 32; ++k) {
-      bf16x8 d[kFragO], x[kFragF];
+    for (int i = 0; i < kFragF; ++i) to.x[i] = operand(&lds_x[buf * kStep * F + x_read[i] + sub * 16 * F], F);
 #pragma unroll
-      for (int i = 0; i < kFragF; ++i) x[i] = operand(&lds_x[buf][x_read[i] + k * 32 * F], F);
+    for (int j = 0; j < kFragO; ++j) to.d[j] = operand(&lds_d[buf * kStep * O + d_read[j] + sub * 16 * O], O);
+  };
+  auto multiply = [&](const Operands& by) {
 #pragma unroll
-      for (int j = 0; j < kFragO; ++j) d[j] = operand(&lds_d[buf][d_read[j] + k * 32 * O], O);
+    for (int i = 0; i < kFragF; ++i)
 #pragma unroll
-      for (int i = 0; i < kFragF; ++i)
-#pragma unroll
-        for (int j = 0; j < kFragO; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], d[j], acc[i][j], 0, 0, 0);
-    }
+      for (int j = 0; j < kFragO; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(by.x[i], by.d[j], acc[i][j], 0, 0, 0);
   };
 
+  // While 16 tokens are multiplied the next 16 tokens' operands come out of LDS; meanwhile the next
+  // step's tile goes into the other buffer, and the tile after that is asked for.  One barrier a
+  // step: behind it the next tile is whole, and nobody reads the present one any more.
+  Operands even, odd;
   if (step_begin < step_end) {
-    fetch(step_begin);
-    stage(0);
+    fetch_d();
+    fetch_x();
+    advance();
+    stage_d(0);
+    stage_x(0);
+    fetch_d();
+    fetch_x();
+    advance();
     __syncthreads();
+    load(even, 0, 0);
     int buf = 0;
     for (uint32_t s = step_begin; s < step_end; ++s, buf ^= 1) {
-      if (s + 1 < step_end) fetch(s + 1);
-      multiply(buf);
-      if (s + 1 < step_end) stage(buf ^ 1);
+      load(odd, buf, 1);
+      multiply(even);
+      load(even, buf, 2);
+      stage_d(buf ^ 1);
+      fetch_d();
+      multiply(odd);
+      load(odd, buf, 3);
+      stage_x(buf ^ 1);
+      fetch_x();
+      advance();
+      multiply(even);
       __syncthreads();
+      load(even, buf ^ 1, 0);
+      multiply(odd);
     }
   }
 
-  // a lane holds features 4 (lane / 16) .. + 3 of each 16, output row lane % 16
+  // Of 32 features x 32 output rows a lane holds output row lane % 32, features 8q + 4 (lane / 32)
+  // .. + 3 for q = 0 .. 3.  Every wavefront turns its 32 rows around in LDS of its own, so that it
+  // stores whole rows; four floats of padding keep the rows on different banks.
+  constexpr int kWide = F / WF, kPitch = kWide + 4;
+  static_assert(WO * WF * 32 * kPitch * 4 <= 2 * kStep * (O + F) * 2, "the turned rows fit the tiles");
+  __syncthreads();
+  float* const turn = reinterpret_cast<float*>(lds) + wave * 32 * kPitch;
+  constexpr int kLanes = kWide / 4;  // lanes per row
+  const int64_t f = f0 + wave_f + (lane % kLanes) * 4;
 #pragma unroll
   for (int j = 0; j < kFragO; ++j) {
-    const int64_t o = o0 + wave_o + j * 16 + (lane & 15);
-    if (o >= a.out_features) continue;
 #pragma unroll
-    for (int i = 0; i < kFragF; ++i) {
-      const int64_t f = f0 + wave_f + i * 16 + (lane >> 4) * 4;
-      if (f >= a.features) continue;
-      if (a.to_partial) {
-        float* p = static_cast<float*>(a.out) + ((int64_t)split * a.out_features + o) * a.pitch + f;
-        *reinterpret_cast<f32x4*>(p) = acc[i][j];
-      } else {
-        store_out4(a, o, f, acc[i][j]);
-      }
+    for (int i = 0; i < kFragF; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(&turn[(lane & 31) * kPitch + i * 32 + q * 8 + (lane >> 5) * 4]) =
+            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll 4
+    for (int r = lane / kLanes; r < 32; r += 64 / kLanes) {
+      const int64_t o = o0 + wave_o + j * 32 + r;
+      const f32x4 v = *reinterpret_cast<const f32x4*>(&turn[r * kPitch + (lane % kLanes) * 4]);
+      if (is_cut)
+        *reinterpret_cast<f32x4*>(a.partial + ((int64_t)slot * O + (wave_o + j * 32 + r)) * F + wave_f +
+                                  (lane % kLanes) * 4) = v;
+      else if (o < a.out_features && f < a.features)
+        store_out4(a, o, f, v);
     }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
 }
 
-// Joins the splits' partial products in their order.
-__global__ __launch_bounds__(256) void wgrad_join_kernel(WgradArgs a, const float* partial) {
-  const uint64_t per_row = (uint64_t)a.pitch / 4;
-  const uint64_t chunks = (uint64_t)a.out_features * per_row;
-  for (uint64_t c = blockIdx.x * 256ull + threadIdx.x; c < chunks; c += gridDim.x * 256ull) {
-    const int64_t o = (int64_t)(c / per_row), f = (int64_t)(c - (uint64_t)o * per_row) * 4;
-    if (f >= a.features) continue;
-    const float* p = partial + (int64_t)c * 4;
-    f32x4 v = *reinterpret_cast<const f32x4*>(p);
-    for (uint32_t s = 1; s < a.splits; ++s)
-      v += *reinterpret_cast<const f32x4*>(p + (int64_t)s * a.out_features * a.pitch);
-    store_out4(a, o, f, v);
-  }
+// Joins the partial products of the cut tiles, in the order of the sum.
+template <int O, int F>
+__global__ __launch_bounds__(256) void wgrad_join_kernel(WgradArgs a) {
+  constexpr uint32_t kPerTile = O * F / 4;
+  const uint32_t at = blockIdx.x * 256 + threadIdx.x, tile = at / kPerTile, in = at % kPerTile;
+  uint32_t tile_o, tile_f;
+  tile_at(a, a.whole + tile, &tile_o, &tile_f);
+  const int64_t o = (int64_t)tile_o * O + in / (F / 4), f = (int64_t)tile_f * F + in % (F / 4) * 4;
+  if (o >= a.out_features || f >= a.features) return;
+  const float* p = a.partial + ((int64_t)tile * kPerTile + in) * 4;
+  f32x4 v = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll 4
+  for (uint32_t s = 1; s < a.splits; ++s)
+    v += *reinterpret_cast<const f32x4*>(p + (int64_t)s * a.cut * O * F);
+  store_out4(a, o, f, v);
 }
 
 // ---------------------------------------------------------------------------
@@ -1037,16 +1138,19 @@ uint32_t column_sum_groups(int64_t rows, int64_t columns) {
 
 // How a weight gradient is cut.
 struct WgradPlan {
-  int parts;       // bf16 parts of the gradient
+  int parts;         // bf16 parts of the gradient
   bool split_first;  // they are written to the workspace
-  int64_t padded;  // row length of the parts
+  int64_t padded;    // row length of the parts
   bool large;
-  uint32_t tiles_o, tiles_f, steps_per_part, steps, splits;
+  uint32_t tiles_o, tiles_f, steps_per_part, steps, whole, cut, splits;
   int64_t parts_bytes, partial_bytes;
 };
 
-WgradPlan plan_wgrad(int64_t rows, int64_t out_features, int64_t features, int64_t pitch,
-                     int64_t grad_stride, int dtype, bool aligned) {
+constexpr int64_t kLarge = 256, kSmall = 128;  // tiles; one large or two small ones fill a CU's LDS
+constexpr int64_t kCUs = 256;
+
+WgradPlan plan_wgrad(int64_t rows, int64_t out_features, int64_t features, int64_t grad_stride,
+                     int dtype, bool aligned) {
   WgradPlan p{};
   p.parts = dtype == TFT_F32 ? 3 : dtype == TFT_F16 ? 2 : 1;
   p.split_first = dtype != TFT_BF16 || !aligned || out_features % 8 || grad_stride % 8 ||
@@ -1055,18 +1159,22 @@ WgradPlan plan_wgrad(int64_t rows, int64_t out_features, int64_t features, int64
   p.parts_bytes = p.split_first ? (p.parts * rows * p.padded * 2 + 255) / 256 * 256 : 0;
   p.steps_per_part = (uint32_t)((rows + kStep - 1) / kStep);
   p.steps = p.steps_per_part * p.parts;
-  const int64_t large_tiles = ((out_features + 255) / 256) * ((features + 255) / 256);
+  const int64_t large_tiles = ((out_features + kLarge - 1) / kLarge) * ((features + kLarge - 1) / kLarge);
   p.large = large_tiles >= 128;
-  const int64_t size = p.large ? 256 : 128;
+  const int64_t size = p.large ? kLarge : kSmall, at_once = p.large ? kCUs : 2 * kCUs;
   p.tiles_o = (uint32_t)((out_features + size - 1) / size);
   p.tiles_f = (uint32_t)((features + size - 1) / size);
+  // whole rounds of the chip take one workgroup per tile; what is left over is cut along the
+  // tokens until it fills the chip too, in pieces of at least four steps
   const int64_t tiles = (int64_t)p.tiles_o * p.tiles_f;
-  const int64_t wanted = p.large ? 256 : 512;
-  int64_t splits = tiles >= wanted ? 1 : wanted / tiles;
+  int64_t cut = tiles % at_once, splits = cut ? at_once / cut : 1;
   const int64_t most = p.steps / 4 > 1 ? p.steps / 4 : 1;
   if (splits > most) splits = most;
+  if (splits == 1) cut = 0;
+  p.whole = (uint32_t)(tiles - cut);
+  p.cut = (uint32_t)cut;
   p.splits = (uint32_t)splits;
-  p.partial_bytes = splits > 1 ? splits * out_features * pitch * 4 : 0;
+  p.partial_bytes = splits * cut * size * size * 4;
   return p;
 }
 
@@ -1240,7 +1348,7 @@ int64_t tft_linear_weight_grad_workspace(const void* grad_out, int64_t rows, int
                                          int64_t features, int64_t grad_row_stride, int64_t pitch,
                                          int dtype) {
   if (rows <= 0 || out_features <= 0 || features <= 0) return 0;
-  const WgradPlan p = plan_wgrad(rows, out_features, features, pitch, grad_row_stride, dtype,
+  const WgradPlan p = plan_wgrad(rows, out_features, features, grad_row_stride, dtype,
                                  (reinterpret_cast<uintptr_t>(grad_out) & 15u) == 0);
   return p.parts_bytes + p.partial_bytes;
 }
@@ -1267,14 +1375,14 @@ int tft_linear_weight_grad(void* grad_weight, void* workspace, int64_t workspace
   }
   if (column_scale && misaligned(column_scale, scale_dtype))
     return fail(TFT_ERR_INVALID_ARGUMENT, "%s: column_scale is misaligned", what);
-  const WgradPlan p = plan_wgrad(rows, out_features, features, pitch, grad_row_stride, dtype,
+  const WgradPlan p = plan_wgrad(rows, out_features, features, grad_row_stride, dtype,
                                  (reinterpret_cast<uintptr_t>(grad_out) & 15u) == 0);
   // offsets within a step's rows are 31 bits
   if (p.padded * 2 * kStep >= (1ll << 31) || pitch * kStep >= (1ll << 31))
     return fail(TFT_ERR_UNSUPPORTED, "%s: rows of %lld gradients or %lld packed values are too long", what,
                 (long long)p.padded, (long long)pitch);
   if ((int64_t)p.steps_per_part * p.parts >= (1ll << 31) ||
-      (int64_t)p.tiles_o * p.tiles_f * p.splits >= (1ll << 31))
+      (int64_t)p.tiles_o * p.tiles_f * 4 >= (1ll << 31))
     return fail(TFT_ERR_UNSUPPORTED, "%s: too many tiles for one grid", what);
   const int64_t needed = p.parts_bytes + p.partial_bytes;
   if (needed && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < needed))
@@ -1294,24 +1402,21 @@ int tft_linear_weight_grad(void* grad_weight, void* workspace, int64_t workspace
     if (int rc = launch(what, k, grid, 256, params, s)) return rc;
     d = a.parts;
   }
-  float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.parts_bytes);
   WgradArgs a{d, static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents), column_scale,
-              p.splits > 1 ? static_cast<void*>(partial) : grad_weight, rows, p.padded, pitch,
-              (uint32_t)out_features, (uint32_t)features, (uint32_t)((features + kBlock - 1) / kBlock),
-              p.tiles_o, p.tiles_f, p.splits, p.steps_per_part, p.steps, scale_dtype, out_dtype,
-              p.splits > 1 ? 1 : 0};
+              grad_weight, reinterpret_cast<float*>(static_cast<char*>(workspace) + p.parts_bytes), rows,
+              p.padded, pitch, (uint32_t)out_features, (uint32_t)features,
+              (uint32_t)((features + kBlock - 1) / kBlock), p.tiles_o, p.tiles_f, p.whole, p.cut, p.splits,
+              p.steps_per_part, p.steps, scale_dtype, out_dtype};
   void* params[] = {&a};
-  const dim3 grid(p.tiles_o * p.tiles_f * p.splits);
-  if (int rc = p.large ? launch(what, TFT_KERNEL(wgrad_kernel<256, 256, 2, 4>), grid, 512, params, s)
-                       : launch(what, TFT_KERNEL(wgrad_kernel<128, 128, 2, 2>), grid, 256, params, s))
+  const dim3 grid(p.whole + p.cut * p.splits);
+  if (int rc = p.large ? launch(what, TFT_KERNEL(wgrad_kernel<kLarge, kLarge, 2, 4>), grid, 512, params, s)
+                       : launch(what, TFT_KERNEL(wgrad_kernel<kSmall, kSmall, 2, 2>), grid, 256, params, s))
     return rc;
-  if (p.splits == 1) return TFT_OK;
-  a.out = grad_weight;
-  const float* from = partial;
-  void* join_params[] = {&a, &from};
-  const uint64_t groups = ((uint64_t)out_features * (pitch / 4) + 255) / 256;
-  return launch(what, TFT_KERNEL(wgrad_join_kernel), dim3((uint32_t)(groups < 16384 ? groups : 16384)), 256,
-                join_params, s);
+  if (!p.cut) return TFT_OK;
+  const int64_t size = p.large ? kLarge : kSmall;
+  const dim3 join((uint32_t)(p.cut * (size * size / 1024)));
+  return p.large ? launch(what, TFT_KERNEL(wgrad_join_kernel<kLarge, kLarge>), join, 256, params, s)
+                 : launch(what, TFT_KERNEL(wgrad_join_kernel<kSmall, kSmall>), join, 256, params, s);
 }
 
 }  // extern "C"
