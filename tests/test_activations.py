@@ -244,11 +244,13 @@ def test_c_entries_refuse_without_a_gpu():
     assert wgrad(out=None) == -1 and wgrad(out=at + 8) == -1 and wgrad(g=None) == -1
     assert wgrad(stride=-64) == -1 and wgrad(o=-1) == -1
     assert wgrad(stride=1 << 25, rows=2) == -2 and b"too long" in err()
-    assert wgrad(t=0, ws_bytes=0) == -1 and b"are needed" in err()
-    assert wgrad(t=0, ws=None) == -1 and wgrad(t=0, ws=at + 8) == -1
+    assert wgrad(o=63, stride=63, ws_bytes=0) == -1 and b"8192 are needed" in err()
+    assert wgrad(o=63, ws=None) == -1 and wgrad(o=63, ws=at + 8) == -1
     assert wgrad(o=0) == 0 and wgrad(features=0, pitch=0) == 0
     space = lib.tft_linear_weight_grad_workspace
-    assert space(at, 64, 64, 130, 64, 144, 1) == 0  # one pass over bf16 rows as they lie
+    for t in range(3):
+        assert space(at, 64, 64, 130, 64, 144, t) == 0  # aligned rows are read as they lie
+    assert space(at, 64, 63, 130, 63, 144, 0) == 64 * 64 * 4
     assert space(at + 2, 64, 64, 130, 64, 144, 1) == 64 * 64 * 2
     assert space(at, 64, 63, 130, 63, 144, 1) == 64 * 64 * 2
     assert space(at, 64, 64, 130, 0, 144, 1) == 64 * 64 * 2  # one row that stands for all

@@ -40,16 +40,37 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
+// 16 or 8 bytes; S: past the caches, for what is not used again soon.  One function per alignment:
+// a template's type parameter would drop it.
+#define TFT_ACCESS(NAME, TYPE)                                      \
+  template <bool S>                                                 \
+  __device__ inline TYPE load_##NAME(const void* p) {               \
+    const TYPE* q = static_cast<const TYPE*>(p);                    \
+    if constexpr (S) return __builtin_nontemporal_load(q);          \
+    return *q;                                                      \
+  }                                                                 \
+  template <bool S>                                                 \
+  __device__ inline void store_##NAME(void* p, TYPE v) {            \
+    TYPE* q = static_cast<TYPE*>(p);                                \
+    if constexpr (S) __builtin_nontemporal_store(v, q);             \
+    else *q = v;                                                    \
+  }
+TFT_ACCESS(16_a2, u32x4_a2)
+TFT_ACCESS(16_a4, u32x4_a4)
+TFT_ACCESS(8, u32x2)
+#undef TFT_ACCESS
+
 // ---------------------------------------------------------------------------
 // Element types: eight consecutive elements of a row as fp32
 // ---------------------------------------------------------------------------
 struct F32 {
   typedef float elem_t;
   typedef struct { u32x4 w[2]; } raw_t;
+  template <bool S>
   __device__ static inline raw_t load(const elem_t* p) {
     raw_t r;
-    r.w[0] = *reinterpret_cast<const u32x4_a4*>(p);
-    r.w[1] = *reinterpret_cast<const u32x4_a4*>(p + 4);
+    r.w[0] = load_16_a4<S>(p);
+    r.w[1] = load_16_a4<S>(p + 4);
     return r;
   }
   __device__ static inline void widen(const raw_t& r, float (&v)[8]) {
@@ -62,9 +83,10 @@ struct F32 {
     for (int i = 0; i < 8; ++i) r.w[i >> 2][i & 3] = __float_as_uint(v[i]);
     return r;
   }
+  template <bool S>
   __device__ static inline void store(elem_t* p, const raw_t& r) {
-    *reinterpret_cast<u32x4_a4*>(p) = r.w[0];
-    *reinterpret_cast<u32x4_a4*>(p + 4) = r.w[1];
+    store_16_a4<S>(p, r.w[0]);
+    store_16_a4<S>(p + 4, r.w[1]);
   }
   __device__ static inline float widen1(elem_t x) { return x; }
   __device__ static inline elem_t narrow1(float x) { return x; }
@@ -75,9 +97,10 @@ struct F32 {
 struct BF16 {
   typedef uint16_t elem_t;
   typedef struct { u32x4 w[1]; } raw_t;
+  template <bool S>
   __device__ static inline raw_t load(const elem_t* p) {
     raw_t r;
-    r.w[0] = *reinterpret_cast<const u32x4_a2*>(p);
+    r.w[0] = load_16_a2<S>(p);
     return r;
   }
   __device__ static inline void widen(const raw_t& r, float (&v)[8]) {
@@ -96,8 +119,9 @@ struct BF16 {
     }
     return r;
   }
+  template <bool S>
   __device__ static inline void store(elem_t* p, const raw_t& r) {
-    *reinterpret_cast<u32x4_a2*>(p) = r.w[0];
+    store_16_a2<S>(p, r.w[0]);
   }
   __device__ static inline float widen1(elem_t x) { return __uint_as_float((uint32_t)x << 16); }
   __device__ static inline elem_t narrow1(float x) {
@@ -109,9 +133,10 @@ struct BF16 {
 struct F16 {
   typedef uint16_t elem_t;
   typedef struct { u32x4 w[1]; } raw_t;
+  template <bool S>
   __device__ static inline raw_t load(const elem_t* p) {
     raw_t r;
-    r.w[0] = *reinterpret_cast<const u32x4_a2*>(p);
+    r.w[0] = load_16_a2<S>(p);
     return r;
   }
   __device__ static inline float widen1(elem_t x) { return __half2float(__ushort_as_half(x)); }
@@ -135,8 +160,9 @@ struct F16 {
       r.w[0][i] = (uint32_t)narrow1(v[2 * i]) | ((uint32_t)narrow1(v[2 * i + 1]) << 16);
     return r;
   }
+  template <bool S>
   __device__ static inline void store(elem_t* p, const raw_t& r) {
-    *reinterpret_cast<u32x4_a2*>(p) = r.w[0];
+    store_16_a2<S>(p, r.w[0]);
   }
   // a packed value may have been rounded up past fp16's largest number
   __device__ static inline float in_range(float x) {
@@ -145,20 +171,20 @@ struct F16 {
 };
 
 // Elements n .. 7 of the eight lie behind the row's end: they are not touched and count as zero.
-template <typename T>
+template <typename T, bool S = false>
 __device__ inline typename T::raw_t load_row(const typename T::elem_t* p, int n) {
-  if (n >= 8) return T::load(p);
+  if (n >= 8) return T::template load<S>(p);
   float v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = i < n ? T::widen1(p[i]) : 0.0f;
   return T::narrow(v);
 }
 
-template <typename T>
+template <typename T, bool S = false>
 __device__ inline void store_row(typename T::elem_t* p, const float (&v)[8], int n) {
   const typename T::raw_t r = T::narrow(v);
   if (n >= 8) {
-    T::store(p, r);
+    T::template store<S>(p, r);
     return;
   }
   constexpr int kPerWord = 4 / sizeof(typename T::elem_t);
@@ -206,18 +232,14 @@ __device__ inline float sum_of_wave(float x) {
   return x;
 }
 
-// Sum over the W wavefronts of a team; every lane gets it.  `part` holds W floats of LDS and
-// must not be in use from an earlier call (the caller alternates between two).
-template <int W>
-__device__ inline float sum_of_team(float x, float* part) {
+// Sum over a workgroup of up to 16 wavefronts; every lane gets it.  `part` holds 16 floats of LDS
+// and must not be in use from an earlier call (the caller alternates between two).
+__device__ inline float sum_of_workgroup(float x, float* part) {
   x = sum_of_wave(x);
-  if constexpr (W > 1) {
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = part[0];
-#pragma unroll
-    for (int i = 1; i < W; ++i) x += part[i];
-  }
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+  __syncthreads();
+  x = part[0];
+  for (uint32_t i = 1; i < blockDim.x / 64; ++i) x += part[i];
   return x;
 }
 
@@ -312,9 +334,11 @@ struct PackArgs {
 
 constexpr int kPackThreads = 256;
 constexpr int kPackUnroll = 4;
+constexpr int kUnpackUnroll = 2;
 constexpr int kPackBlocks = kPackThreads / 16 * kPackUnroll;  // blocks per workgroup
+constexpr int kUnpackBlocks = kPackThreads / 16 * kUnpackUnroll;
 
-template <typename T>
+template <typename T, bool S>
 __global__ __launch_bounds__(kPackThreads) void pack_kernel(PackArgs a) {
   const int lane = threadIdx.x & 15;
   const uint32_t first = blockIdx.x * (uint32_t)kPackBlocks + (threadIdx.x >> 4);
@@ -328,7 +352,7 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(PackArgs a) {
     row[u] = divide(min(b, a.blocks - 1), a.per_row);
     col[u] = (int64_t)(min(b, a.blocks - 1) - row[u] * a.per_row.d) * kBlock + lane * 8;
     const int64_t left = b < a.blocks ? a.features - col[u] : 0;
-    raw[u] = load_row<T>(x + (int64_t)row[u] * a.row_stride + col[u], (int)min(left, (int64_t)8));
+    raw[u] = load_row<T, S>(x + (int64_t)row[u] * a.row_stride + col[u], (int)min(left, (int64_t)8));
   }
 #pragma unroll
   for (int u = 0; u < kPackUnroll; ++u) {
@@ -354,17 +378,17 @@ struct UnpackArgs {
   Divider per_row;
 };
 
-// S: type of the column scale
-template <typename T, typename S>
+// W: type of the column scale
+template <typename T, typename W, bool S>
 __global__ __launch_bounds__(kPackThreads) void unpack_kernel(UnpackArgs a) {
   const int lane = threadIdx.x & 15;
-  const uint32_t first = blockIdx.x * (uint32_t)kPackBlocks + (threadIdx.x >> 4);
+  const uint32_t first = blockIdx.x * (uint32_t)kUnpackBlocks + (threadIdx.x >> 4);
   typename T::elem_t* out = static_cast<typename T::elem_t*>(a.out);
-  u32x2 q[kPackUnroll];
-  uint32_t e[kPackUnroll], row[kPackUnroll];
-  int64_t col[kPackUnroll];
+  u32x2 q[kUnpackUnroll];
+  uint32_t e[kUnpackUnroll], row[kUnpackUnroll];
+  int64_t col[kUnpackUnroll];
 #pragma unroll
-  for (int u = 0; u < kPackUnroll; ++u) {
+  for (int u = 0; u < kUnpackUnroll; ++u) {
     const uint32_t b = min(first + u * (kPackThreads / 16), a.blocks - 1);
     row[u] = divide(b, a.per_row);
     col[u] = (int64_t)(b - row[u] * a.per_row.d) * kBlock + lane * 8;
@@ -374,7 +398,7 @@ __global__ __launch_bounds__(kPackThreads) void unpack_kernel(UnpackArgs a) {
     e[u] = a.exponents[b];
   }
 #pragma unroll
-  for (int u = 0; u < kPackUnroll; ++u) {
+  for (int u = 0; u < kUnpackUnroll; ++u) {
     if (first + u * (kPackThreads / 16) >= a.blocks) return;
     const int n = (int)min(a.features - col[u], (int64_t)8);
     if (n <= 0) continue;
@@ -382,14 +406,14 @@ __global__ __launch_bounds__(kPackThreads) void unpack_kernel(UnpackArgs a) {
     dequantise(q[u], scale_of(e[u]), v);
     if (a.column_scale) {
       float w[8];
-      load_weight<S>(a.column_scale, false, col[u], n, w);
+      load_weight<W>(a.column_scale, false, col[u], n, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] *= w[i];
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = T::in_range(v[i]);
     }
-    store_row<T>(out + (int64_t)row[u] * a.features + col[u], v, n);
+    store_row<T, S>(out + (int64_t)row[u] * a.features + col[u], v, n);
   }
 }
 
@@ -412,16 +436,19 @@ struct NormArgs {
   float eps;
 };
 
-// One team of W wavefronts per row, C times eight features per lane: the row is read once and
-// stays in registers between the sum of squares and the outputs.  W = 1 runs four rows per
-// workgroup without a barrier.
-template <typename T, int W, int C>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_kernel(NormArgs a) {
-  constexpr int kTeam = 64 * W;
-  __shared__ float part[W];
+// The row is read once and stays in registers between the sum of squares and the outputs.  Up to
+// 512 features are one wavefront's, four rows to a workgroup and no barrier (Four); longer rows
+// take a workgroup of as many wavefronts as it has 512 features, from 8192 on twice as many
+// features a lane (C = 2).  One chunk of eight features a lane keeps the most wavefronts, and so
+// the most loads, in flight: 16384 x 4096 bf16 with a residual takes 97.7 us with eight
+// wavefronts of one chunk, 101 with four of two, 104 with two of four.
+template <typename T, bool Four, int C, bool S>
+__global__ __launch_bounds__(Four ? 256 : 1024) void norm_kernel(NormArgs a) {
+  const int kTeam = Four ? 64 : blockDim.x;
+  __shared__ float part[Four ? 1 : 16];
   typedef typename T::elem_t elem_t;
-  const int lane = W == 1 ? (threadIdx.x & 63) : threadIdx.x;
-  const uint32_t row = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  const int lane = Four ? (threadIdx.x & 63) : threadIdx.x;
+  const uint32_t row = Four ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (row >= a.rows) return;  // whole teams
   const elem_t* x = static_cast<const elem_t*>(a.x) + (int64_t)row * a.x_stride;
   float h[C][8];
@@ -430,14 +457,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_kernel(NormArgs a)
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int col = (c * kTeam + lane) * 8;
-      rx[c] = load_row<T>(x + col, a.features - col);
+      rx[c] = load_row<T, S>(x + col, a.features - col);
     }
     if (a.residual) {
       const elem_t* r = static_cast<const elem_t*>(a.residual) + (int64_t)row * a.residual_stride;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int col = (c * kTeam + lane) * 8;
-        rr[c] = load_row<T>(r + col, a.features - col);
+        rr[c] = load_row<T, S>(r + col, a.features - col);
       }
 #pragma unroll
       for (int c = 0; c < C; ++c) {
@@ -450,7 +477,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_kernel(NormArgs a)
         // what is normed is the sum as it is stored: the layer's other readers see that one
         T::widen(T::narrow(h[c]), h[c]);
         if (col < a.features)
-          store_row<T>(static_cast<elem_t*>(a.h) + (int64_t)row * a.features + col, h[c],
+          store_row<T, S>(static_cast<elem_t*>(a.h) + (int64_t)row * a.features + col, h[c],
                        a.features - col);
       }
     } else {
@@ -463,7 +490,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_kernel(NormArgs a)
   for (int c = 0; c < C; ++c)
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = fmaf(h[c][i], h[c][i], ss);
-  ss = sum_of_team<W>(ss, part);
+  ss = Four ? sum_of_wave(ss) : sum_of_workgroup(ss, part);
   const float rstd = 1.0f / sqrtf(ss / (float)a.features + a.eps);
   if (a.rstd && lane == 0) a.rstd[row] = rstd;
   const int blocks = (a.features + kBlock - 1) / kBlock;
@@ -483,7 +510,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_kernel(NormArgs a)
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = h[c][i];
     }
-    if (n > 0) store_row<T>(static_cast<elem_t*>(a.y) + (int64_t)row * a.features + col, y, n);
+    if (n > 0) store_row<T, S>(static_cast<elem_t*>(a.y) + (int64_t)row * a.features + col, y, n);
     if (a.values) {
       if (n < 8) {  // 0 times an infinite rstd is no zero
 #pragma unroll
@@ -493,7 +520,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_kernel(NormArgs a)
       int e;
       const u32x2 q = quantise(h[c], &e);
       if (col < a.pitch)
-        *reinterpret_cast<u32x2*>(a.values + (int64_t)row * a.pitch + col) = q;
+        store_8<S>(a.values + (int64_t)row * a.pitch + col, q);
       if ((lane & 15) == 0) a.exponents[(int64_t)row * blocks + col / kBlock] = (uint8_t)e;
     }
   }
@@ -514,93 +541,103 @@ struct NormBackArgs {
   int weight_is_f32;
 };
 
-// The workgroup takes rows blockIdx.x, + gridDim.x, ... (four at a time for W = 1) and keeps the
+// Teams as in norm_kernel.  A workgroup takes rows blockIdx.x, + gridDim.x, ... and keeps the
 // weight gradient of its rows in registers; column_reduce_kernel adds the workgroups' partial
-// sums in a fixed order.
-template <typename T, int W, int C>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_back_kernel(NormBackArgs a) {
-  constexpr int kTeam = 64 * W;
-  constexpr int kRows = W == 1 ? 4 : 1;
-  __shared__ float part[2][W];
-  __shared__ float gathered[W == 1 ? 3 : 1][W == 1 ? 64 * C * 8 : 1];
+// sums in a fixed order.  A row is asked for while the one before it is worked on: few rows are
+// in flight, because every workgroup leaves a partial sum of a whole row behind.
+template <typename T, bool Four, int C>
+__global__ __launch_bounds__(Four ? 256 : 1024) void norm_back_kernel(NormBackArgs a) {
+  constexpr int kRows = Four ? 4 : 1;
+  constexpr bool kAhead = C == 1;  // two rows of two chunks do not fit 16 wavefronts' registers
+  const int kTeam = Four ? 64 : blockDim.x;
+  __shared__ float part[2][16];
+  __shared__ float gathered[Four ? 3 : 1][Four ? 64 * C * 8 : 1];
   typedef typename T::elem_t elem_t;
-  const int lane = W == 1 ? (threadIdx.x & 63) : threadIdx.x;
-  const int team = W == 1 ? (threadIdx.x >> 6) : 0;
+  const int lane = Four ? (threadIdx.x & 63) : threadIdx.x;
+  const int team = Four ? (threadIdx.x >> 6) : 0;
   const int blocks = (a.features + kBlock - 1) / kBlock;
   const float inv_n = 1.0f / (float)a.features;
-  float gw[C][8];
+  float gw[C][8], w[C][8];
 #pragma unroll
-  for (int c = 0; c < C; ++c)
+  for (int c = 0; c < C; ++c) {
+    const int col = (c * kTeam + lane) * 8;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) gw[c][i] = 0.0f;
-  int turn = 0;
-  for (uint32_t row = blockIdx.x * kRows + team; row < a.rows; row += gridDim.x * kRows, turn ^= 1) {
-    typename T::raw_t rg[C];
-    u32x2 rq[C];
-    uint32_t re[C];
+    for (int i = 0; i < 8; ++i) gw[c][i] = 0.0f, w[c][i] = 1.0f;
+    if (a.weight && col < a.features) load_weight<T>(a.weight, a.weight_is_f32, col, a.features - col, w[c]);
+  }
+  struct Row {
+    typename T::raw_t gy[C], gh[C];
+    u32x2 q[C];
+    uint32_t e[C];
+    float rstd;
+  };
+  auto ask = [&](Row& r, uint32_t row) {
     const elem_t* gy = static_cast<const elem_t*>(a.grad_y) + (int64_t)row * a.grad_y_stride;
+    const elem_t* gh = static_cast<const elem_t*>(a.grad_h) + (int64_t)row * a.grad_h_stride;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int col = (c * kTeam + lane) * 8;
-      rg[c] = load_row<T>(gy + col, a.features - col);
-      rq[c] = u32x2{0, 0};
-      re[c] = 0;
-      if (col < a.pitch) {
-        rq[c] = *reinterpret_cast<const u32x2*>(a.values + (int64_t)row * a.pitch + col);
-        if (col < a.features) re[c] = a.exponents[(int64_t)row * blocks + col / kBlock];
+      r.gy[c] = load_row<T>(gy + col, a.features - col);
+      r.q[c] = u32x2{0, 0};
+      r.e[c] = 0;
+      if (col < a.features) {
+        r.q[c] = *reinterpret_cast<const u32x2*>(a.values + (int64_t)row * a.pitch + col);
+        r.e[c] = a.exponents[(int64_t)row * blocks + col / kBlock];
       }
+      if (a.grad_h) r.gh[c] = load_row<T>(gh + col, a.features - col);
     }
-    const float rstd = a.rstd[row];
+    r.rstd = a.rstd[row];
+  };
+  int turn = 0;
+  const uint32_t step = gridDim.x * kRows;
+  uint32_t row = blockIdx.x * kRows + team;
+  Row next;
+  if (kAhead && row < a.rows) ask(next, row);
+  for (; row < a.rows; turn ^= 1) {
+    if (!kAhead) ask(next, row);
+    const Row r = next;
+    const uint32_t here = row;
+    row = a.rows - row > step ? row + step : a.rows;
+    if (kAhead && row < a.rows) ask(next, row);
     float n[C][8], g[C][8];
     float dot = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int col = (c * kTeam + lane) * 8;
-      float gyv[8];
-      dequantise(rq[c], scale_of(re[c]), n[c]);
+      dequantise(r.q[c], scale_of(r.e[c]), n[c]);
       if (a.features - col < 8) {  // what a caller's padding holds does not count
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (i >= a.features - col) n[c][i] = 0.0f;
       }
-      T::widen(rg[c], gyv);
-      if (a.weight && col < a.features) {
-        load_weight<T>(a.weight, a.weight_is_f32, col, a.features - col, g[c]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[c][i] *= gyv[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[c][i] = gyv[i];
-      }
+      T::widen(r.gy[c], g[c]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        gw[c][i] = fmaf(gyv[i], n[c][i], gw[c][i]);
+        gw[c][i] = fmaf(g[c][i], n[c][i], gw[c][i]);
+        g[c][i] *= w[c][i];
         dot = fmaf(g[c][i], n[c][i], dot);
       }
     }
-    dot = sum_of_team<W>(dot, part[turn]) * inv_n;
+    dot = (Four ? sum_of_wave(dot) : sum_of_workgroup(dot, part[turn])) * inv_n;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int col = (c * kTeam + lane) * 8;
       if (col >= a.features) break;
       float gx[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) gx[i] = rstd * fmaf(-n[c][i], dot, g[c][i]);
+      for (int i = 0; i < 8; ++i) gx[i] = r.rstd * fmaf(-n[c][i], dot, g[c][i]);
       if (a.grad_h) {
         float gh[8];
-        T::widen(load_row<T>(static_cast<const elem_t*>(a.grad_h) +
-                                 (int64_t)row * a.grad_h_stride + col,
-                             a.features - col),
-                 gh);
+        T::widen(r.gh[c], gh);
 #pragma unroll
         for (int i = 0; i < 8; ++i) gx[i] += gh[i];
       }
-      store_row<T>(static_cast<elem_t*>(a.grad_x) + (int64_t)row * a.features + col, gx,
-                   a.features - col);
+      store_row<T>(static_cast<elem_t*>(a.grad_x) + (int64_t)here * a.features + col, gx,
+                      a.features - col);
     }
   }
   if (!a.partial) return;
-  if constexpr (W == 1) {  // the four wavefronts' sums, in their order
+  if constexpr (Four) {  // the four wavefronts' sums, in their order
     if (team) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
@@ -645,7 +682,7 @@ __global__ __launch_bounds__(1024) void column_reduce_kernel(const float* partia
 }
 
 // Partial column sums of a [rows, columns] matrix: 256 lanes of eight columns, rows
-// blockIdx.y, + gridDim.y, ...
+// blockIdx.y, + gridDim.y, ..., four of them in flight.
 template <typename T>
 __global__ __launch_bounds__(256) void column_sum_kernel(const void* x, float* partial, uint32_t rows,
                                                          int64_t columns, int64_t stride) {
@@ -654,12 +691,20 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const void* x, float* p
   const int n = (int)min(columns - col, (int64_t)8);
   const typename T::elem_t* p = static_cast<const typename T::elem_t*>(x) + col;
   float s[8] = {};
-#pragma unroll 4
-  for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    float v[8];
-    T::widen(load_row<T>(p + (int64_t)r * stride, n), v);
+  for (uint64_t r = blockIdx.y; r < rows; r += 4ull * gridDim.y) {
+    typename T::raw_t raw[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] += v[i];
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t at = r + (uint64_t)k * gridDim.y;
+      raw[k] = load_row<T>(p + (int64_t)min(at, (uint64_t)rows - 1) * stride, at < rows ? n : 0);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float v[8];
+      T::widen(raw[k], v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += v[i];
+    }
   }
   store_row<F32>(partial + (int64_t)blockIdx.y * columns + col, s, n);
 }
@@ -667,30 +712,34 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const void* x, float* p
 // ---------------------------------------------------------------------------
 // Weight gradient of a linear layer:  G[o][f] = w[f] * sum_t D[t][o] X[t][f]
 // ---------------------------------------------------------------------------
-// The products run on the bf16 matrix cores.  X is exact in bf16, and D is split into bf16
-// parts that add up to it exactly: one part for bf16, two for fp16 (11 bits), three for fp32
-// (24 bits).  The parts lie behind one another along t, so the kernel sees one longer sum.
-// Written where D is not bf16 already, or its rows do not start at 16-byte boundaries.
-struct SplitArgs {
-  const void* d;
-  uint16_t* parts;  // [n_parts][rows][padded]
-  int64_t rows, columns, stride, padded;
-  uint64_t chunks;  // rows * padded / 8
+// The products run on the bf16 matrix cores.  X is exact in bf16, and D is split into bf16 parts
+// that add up to it exactly while it goes into LDS: one part for bf16, two for fp16 (11 bits),
+// three for fp32 (24 bits).  Every part is multiplied with the same X.
+template <typename T>
+struct Parts;
+template <>
+struct Parts<BF16> {
+  static constexpr int kParts = 1, kTokens = 64;  // tokens of one step: with all parts of D and X
+};                                                // twice, a step's tiles fill the LDS
+template <>
+struct Parts<F16> {
+  static constexpr int kParts = 2, kTokens = 32;
+};
+template <>
+struct Parts<F32> {
+  static constexpr int kParts = 3, kTokens = 32;
 };
 
-template <typename T, int P>
-__global__ __launch_bounds__(256) void split_kernel(SplitArgs a) {
-  const int64_t per_row = a.padded / 8;
-  for (uint64_t c = blockIdx.x * 256ull + threadIdx.x; c < a.chunks; c += gridDim.x * 256ull) {
-    const int64_t row = (int64_t)(c / (uint64_t)per_row);
-    const int64_t col = (int64_t)(c - (uint64_t)row * per_row) * 8;
+// Eight elements -> their parts, eight bf16 each
+template <typename T>
+__device__ inline void split(const typename T::raw_t& raw, u32x4 (&part)[Parts<T>::kParts]) {
+  if constexpr (Parts<T>::kParts == 1) {
+    part[0] = raw.w[0];
+  } else {
     float v[8];
-    T::widen(load_row<T>(static_cast<const typename T::elem_t*>(a.d) + row * a.stride + col,
-                         (int)min(a.columns - col, (int64_t)8)),
-             v);
+    T::widen(raw, v);
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      u32x4 w;
+    for (int p = 0; p < Parts<T>::kParts; ++p) {
       uint32_t b[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -700,16 +749,36 @@ __global__ __launch_bounds__(256) void split_kernel(SplitArgs a) {
         v[i] = (b[i] & 0x7fffffffu) == kInfBits ? 0.0f : v[i] - cut;
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = (b[2 * i] >> 16) | (b[2 * i + 1] & 0xffff0000u);
-      *reinterpret_cast<u32x4*>(a.parts + ((int64_t)p * a.rows + row) * a.padded + col) = w;
+      for (int i = 0; i < 4; ++i) part[p][i] = (b[2 * i] >> 16) | (b[2 * i + 1] & 0xffff0000u);
     }
   }
 }
 
-constexpr int kStep = 64;  // tokens per step of the product
+// D with rows that start at multiples of 16 bytes and are whole chunks of eight, where the
+// caller's are not
+struct AlignArgs {
+  const void* d;
+  void* aligned;  // [rows][padded]
+  int64_t columns, stride, padded;
+  uint64_t chunks;  // rows * padded / 8
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void align_kernel(AlignArgs a) {
+  typedef typename T::elem_t elem_t;
+  const uint64_t per_row = (uint64_t)a.padded / 8;
+  for (uint64_t c = blockIdx.x * 256ull + threadIdx.x; c < a.chunks; c += gridDim.x * 256ull) {
+    const uint64_t row = c / per_row;
+    const int64_t col = (int64_t)(c - row * per_row) * 8;
+    T::template store<false>(
+        static_cast<elem_t*>(a.aligned) + c * 8,
+        load_row<T>(static_cast<const elem_t*>(a.d) + (int64_t)row * a.stride + col,
+                    (int)min(a.columns - col, (int64_t)8)));
+  }
+}
 
 struct WgradArgs {
-  const uint16_t* d;  // bf16 parts [n_parts][rows][d_stride]
+  const void* d;  // [rows][d_stride]
   const uint8_t* values;
   const uint8_t* exponents;
   const void* column_scale;  // or NULL
@@ -718,9 +787,9 @@ struct WgradArgs {
   int64_t rows, d_stride, pitch;
   uint32_t out_features, features, blocks;
   uint32_t tiles_o, tiles_f;
-  uint32_t whole, cut, splits;     // tiles of one workgroup each, tiles of `splits` workgroups each
-  uint32_t steps_per_part, steps;  // of all parts
-  int scale_type, out_type;        // TFT_F32 ...
+  uint32_t whole, cut, splits;  // tiles of one workgroup each, tiles of `splits` workgroups each
+  uint32_t steps;
+  int scale_type, out_type;  // TFT_F32 ...
 };
 
 // Workgroup ids go round the 8 XCDs in turn; this gives each of them a run of neighbouring
@@ -794,15 +863,17 @@ __device__ inline void store_out4(const WgradArgs& a, int64_t o, int64_t f, f32x
 // read together, lie on different banks.
 __device__ inline int spread(int t) { return (t & 3) | ((t & 1) << 2); }
 
-template <int O, int F, int WO, int WF>
+template <typename T, int O, int F, int WO, int WF>
 __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
-  constexpr int kThreads = 64 * WO * WF;
-  constexpr int kDChunks = kStep * O / 8 / kThreads;   // 16-byte chunks of D per thread and step
-  constexpr int kXChunks = kStep * F / 16 / kThreads;  // 16-byte chunks of X
+  typedef typename T::elem_t elem_t;
+  constexpr int kThreads = 64 * WO * WF, kParts = Parts<T>::kParts, kTokens = Parts<T>::kTokens;
+  constexpr int kDChunks = kTokens * O / 8 / kThreads;   // chunks of eight elements of D per thread and step
+  constexpr int kXChunks = kTokens * F / 16 / kThreads;  // 16-byte chunks of X
+  constexpr int kDTile = kParts * kTokens * O, kXTile = kTokens * F;
   constexpr int kFragO = O / WO / 32, kFragF = F / WF / 32;
-  __shared__ __attribute__((aligned(128))) uint16_t lds[2 * kStep * (O + F)];
-  uint16_t* const lds_d = lds;                  // two tiles of kStep x O
-  uint16_t* const lds_x = lds + 2 * kStep * O;  // two tiles of kStep x F
+  __shared__ __attribute__((aligned(128))) uint16_t lds[2 * (kDTile + kXTile)];
+  uint16_t* const lds_d = lds;               // two tiles, [part][token][O]
+  uint16_t* const lds_x = lds + 2 * kDTile;  // two tiles, [token][F]
 
   const bool is_cut = blockIdx.x >= a.whole;
   uint32_t tile_o, tile_f, slot = 0, step_begin = 0, step_end = a.steps;
@@ -822,7 +893,7 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
 #pragma unroll
   for (int i = 0; i < kDChunks; ++i) {
     const int c = i * kThreads + threadIdx.x, t = c / (O / 8), j = c % (O / 8);
-    d_off[i] = o0 + j * 8 < a.out_features ? (uint32_t)((t * a.d_stride + j * 8) * 2) : 0x80000000u;
+    d_off[i] = o0 + j * 8 < a.out_features ? (uint32_t)((t * a.d_stride + j * 8) * sizeof(elem_t)) : 0x80000000u;
     d_lds[i] = t * O + (((j >> 1) ^ spread(t)) << 4) + ((j & 1) << 3);
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -846,33 +917,27 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
   for (int f = 0; f < kFragF; ++f)
     x_read[f] = t_lane * F + (((wave_f / 16 + 2 * f + ((lane >> 4) & 1)) ^ spread(t_lane)) << 4) + ((lane & 3) << 2);
 
-  // the staged tile of one step: d, x and e point at its first token and column
-  const uint16_t* d_at;
-  const uint8_t *x_at, *e_at;
-  int64_t left;  // tokens from there on
-  {
-    const uint32_t part = step_begin / a.steps_per_part;
-    const int64_t t0 = (int64_t)(step_begin - part * a.steps_per_part) * kStep;
-    d_at = a.d + ((int64_t)part * a.rows + t0) * a.d_stride + o0;
-    x_at = a.values + t0 * a.pitch + f0;
-    e_at = a.exponents + t0 * a.blocks + f0 / kBlock;
-    left = a.rows - t0;
-  }
-  uint32_t to_fetch = step_end - step_begin;
-  u32x4 d_reg[kDChunks], x_reg[kXChunks];
+  // the tile of the next step to ask for: d, x and e point at its first token and column
+  const int64_t t0 = (int64_t)step_begin * kTokens;
+  const elem_t* d_at = static_cast<const elem_t*>(a.d) + t0 * a.d_stride + o0;
+  const uint8_t* x_at = a.values + t0 * a.pitch + f0;
+  const uint8_t* e_at = a.exponents + t0 * a.blocks + f0 / kBlock;
+  int64_t left = min(a.rows, (int64_t)step_end * kTokens) - t0;  // tokens from there on; may pass below 0
+  typename T::raw_t d_reg[kDChunks];
+  u32x4 x_reg[kXChunks];
   uint32_t e_reg[kXChunks];
   // D and X are asked for at different times, each as soon as its registers are free
   auto fetch_d = [&]() {
-    const int64_t rows = to_fetch ? left : 0;  // nothing is read behind the last step
-    const auto d = buffer(d_at, (rows * a.d_stride - o0) * 2);
+    const auto d = buffer(d_at, (left * a.d_stride - o0) * (int64_t)sizeof(elem_t));
 #pragma unroll
     for (int i = 0; i < kDChunks; ++i)
-      d_reg[i] = __builtin_amdgcn_raw_buffer_load_b128(d, d_off[i], 0, 0);
+#pragma unroll
+      for (int w = 0; w < (int)sizeof(elem_t) / 2; ++w)
+        d_reg[i].w[w] = __builtin_amdgcn_raw_buffer_load_b128(d, d_off[i] + 16 * w, 0, 0);
   };
   auto fetch_x = [&]() {
-    const int64_t rows = to_fetch ? left : 0;
-    const auto x = buffer(x_at, rows * a.pitch - f0);
-    const auto e = buffer(e_at, rows * a.blocks - f0 / kBlock);
+    const auto x = buffer(x_at, left * a.pitch - f0);
+    const auto e = buffer(e_at, left * a.blocks - f0 / kBlock);
 #pragma unroll
     for (int i = 0; i < kXChunks; ++i) {
       x_reg[i] = __builtin_amdgcn_raw_buffer_load_b128(x, x_off[i], 0, 0);
@@ -880,22 +945,20 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
     }
   };
   auto advance = [&]() {
-    to_fetch -= to_fetch ? 1 : 0;
-    left -= kStep;
-    d_at += kStep * a.d_stride;
-    x_at += kStep * a.pitch;
-    e_at += (int64_t)kStep * a.blocks;
-    if (left <= 0) {  // the next part starts behind this one's last row, X over again
-      d_at += left * a.d_stride;
-      x_at += (left - a.rows) * a.pitch;
-      e_at += (left - a.rows) * a.blocks;
-      left = a.rows;
-    }
+    left -= kTokens;
+    d_at += kTokens * a.d_stride;
+    x_at += kTokens * a.pitch;
+    e_at += (int64_t)kTokens * a.blocks;
   };
   auto stage_d = [&](int buf) {
 #pragma unroll
-    for (int i = 0; i < kDChunks; ++i)
-      *reinterpret_cast<u32x4*>(&lds_d[buf * kStep * O + d_lds[i]]) = d_reg[i];
+    for (int i = 0; i < kDChunks; ++i) {
+      u32x4 part[kParts];
+      split<T>(d_reg[i], part);
+#pragma unroll
+      for (int p = 0; p < kParts; ++p)
+        *reinterpret_cast<u32x4*>(&lds_d[buf * kDTile + p * kTokens * O + d_lds[i]]) = part[p];
+    }
   };
   auto stage_x = [&](int buf) {
 #pragma unroll
@@ -912,8 +975,8 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
           half[h][2 * w + 1] = __builtin_bit_cast(
               uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(from, scale, true));
         }
-      *reinterpret_cast<u32x4*>(&lds_x[buf * kStep * F + x_lds[i]]) = half[0];
-      *reinterpret_cast<u32x4*>(&lds_x[buf * kStep * F + (x_lds[i] ^ 8)]) = half[1];
+      *reinterpret_cast<u32x4*>(&lds_x[buf * kXTile + x_lds[i]]) = half[0];
+      *reinterpret_cast<u32x4*>(&lds_x[buf * kXTile + (x_lds[i] ^ 8)]) = half[1];
     }
   };
 
@@ -933,27 +996,32 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
     const s16x4 lo = read_tr(base), hi = read_tr(base + 4 * columns);
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  struct Operands {
-    bf16x8 d[kFragO], x[kFragF];
-  };
-  auto load = [&](Operands& to, int buf, int sub) {  // tokens 16 sub .. + 15
+  // A step's products: kTokens / 16 groups of tokens, every part of D with the same X
+  constexpr int kProducts = kTokens / 16 * kParts;
+  bf16x8 d[2][kFragO], x[2][kFragF];
+  auto load = [&](int product, int buf) {
+    const int group = product / kParts, part = product % kParts;
+    if (part == 0)
 #pragma unroll
-    for (int i = 0; i < kFragF; ++i) to.x[i] = operand(&lds_x[buf * kStep * F + x_read[i] + sub * 16 * F], F);
+      for (int i = 0; i < kFragF; ++i)
+        x[group & 1][i] = operand(&lds_x[buf * kXTile + x_read[i] + group * 16 * F], F);
 #pragma unroll
-    for (int j = 0; j < kFragO; ++j) to.d[j] = operand(&lds_d[buf * kStep * O + d_read[j] + sub * 16 * O], O);
+    for (int j = 0; j < kFragO; ++j)
+      d[product & 1][j] = operand(&lds_d[buf * kDTile + d_read[j] + (part * kTokens + group * 16) * O], O);
   };
-  auto multiply = [&](const Operands& by) {
+  auto multiply = [&](int product) {
 #pragma unroll
     for (int i = 0; i < kFragF; ++i)
 #pragma unroll
       for (int j = 0; j < kFragO; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(by.x[i], by.d[j], acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[product / kParts & 1][i], d[product & 1][j],
+                                                            acc[i][j], 0, 0, 0);
   };
 
-  // While 16 tokens are multiplied the next 16 tokens' operands come out of LDS; meanwhile the next
-  // step's tile goes into the other buffer, and the tile after that is asked for.  One barrier a
-  // step: behind it the next tile is whole, and nobody reads the present one any more.
-  Operands even, odd;
+  // While one product runs, the next one's operands come out of LDS; meanwhile the next step's
+  // tile goes into the other buffer, and the tile after that is asked for.  One barrier a step:
+  // behind it the next tile is whole, and nobody reads the present one any more.
+  static_assert(kProducts % 2 == 0 && kTokens / 16 % 2 == 0, "the operands' turns close with a step");
   if (step_begin < step_end) {
     fetch_d();
     fetch_x();
@@ -964,23 +1032,26 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
     fetch_x();
     advance();
     __syncthreads();
-    load(even, 0, 0);
+    load(0, 0);
     int buf = 0;
     for (uint32_t s = step_begin; s < step_end; ++s, buf ^= 1) {
-      load(odd, buf, 1);
-      multiply(even);
-      load(even, buf, 2);
-      stage_d(buf ^ 1);
-      fetch_d();
-      multiply(odd);
-      load(odd, buf, 3);
-      stage_x(buf ^ 1);
-      fetch_x();
-      advance();
-      multiply(even);
+#pragma unroll
+      for (int k = 0; k + 1 < kProducts; ++k) {
+        load(k + 1, buf);
+        if (k == 1) {
+          stage_d(buf ^ 1);
+          fetch_d();
+        }
+        if (k == 2) {
+          stage_x(buf ^ 1);
+          fetch_x();
+          advance();
+        }
+        multiply(k);
+      }
       __syncthreads();
-      load(even, buf ^ 1, 0);
-      multiply(odd);
+      load(0, buf ^ 1);
+      multiply(kProducts - 1);
     }
   }
 
@@ -988,7 +1059,7 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
   // .. + 3 for q = 0 .. 3.  Every wavefront turns its 32 rows around in LDS of its own, so that it
   // stores whole rows; four floats of padding keep the rows on different banks.
   constexpr int kWide = F / WF, kPitch = kWide + 4;
-  static_assert(WO * WF * 32 * kPitch * 4 <= 2 * kStep * (O + F) * 2, "the turned rows fit the tiles");
+  static_assert(WO * WF * 32 * kPitch * 4 <= (int)sizeof(lds), "the turned rows fit the tiles");
   __syncthreads();
   float* const turn = reinterpret_cast<float*>(lds) + wave * 32 * kPitch;
   constexpr int kLanes = kWide / 4;  // lanes per row
@@ -1005,7 +1076,8 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll 4
-    for (int r = lane / kLanes; r < 32; r += 64 / kLanes) {
+    for (int k = 0; k < kLanes / 2; ++k) {
+      const int r = k * (64 / kLanes) + lane / kLanes;
       const int64_t o = o0 + wave_o + j * 32 + r;
       const f32x4 v = *reinterpret_cast<const f32x4*>(&turn[r * kPitch + (lane % kLanes) * 4]);
       if (is_cut)
@@ -1040,6 +1112,11 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(WgradArgs a) {
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
+// A call that moves more than the last-level cache holds reads and writes past the caches: packing
+// 224 MiB of bf16 takes 54 us so and 62 through them, unpacking 56 and 60, the norm of two times
+// 128 MiB 99 and 107.  Below, what a call leaves in the cache is worth more to the next one:
+// unpacking 128 MiB and summing it takes 62 us past the caches and 57 through them.
+constexpr int64_t kLastLevelCache = 256ll << 20;
 constexpr int64_t kMostRows = 1ll << 31;
 constexpr int kMostNormFeatures = 16384;
 
@@ -1086,23 +1163,26 @@ int launch(const char* what, const void* kernel, dim3 grid, int threads, void** 
 
 #define TFT_KERNEL(...) reinterpret_cast<const void*>(&__VA_ARGS__)
 
-template <typename T>
+// Threads of a workgroup for rows of so many features, `chunks` of eight a lane
+int norm_threads(int features, int chunks) { return (features + 512 * chunks - 1) / (512 * chunks) * 64; }
+
+template <typename T, bool S>
 int launch_norm(const char* what, const NormArgs& a, hipStream_t s) {
   NormArgs args = a;
   void* params[] = {&args};
-  const dim3 four((a.rows + 3) / 4), one(a.rows);
-  if (a.features <= 512) return launch(what, TFT_KERNEL(norm_kernel<T, 1, 1>), four, 256, params, s);
-  if (a.features <= 1024) return launch(what, TFT_KERNEL(norm_kernel<T, 1, 2>), four, 256, params, s);
-  if (a.features <= 2048) return launch(what, TFT_KERNEL(norm_kernel<T, 4, 1>), one, 256, params, s);
-  if (a.features <= 4096) return launch(what, TFT_KERNEL(norm_kernel<T, 4, 2>), one, 256, params, s);
-  if (a.features <= 8192) return launch(what, TFT_KERNEL(norm_kernel<T, 4, 4>), one, 256, params, s);
-  return launch(what, TFT_KERNEL(norm_kernel<T, 8, 4>), one, 512, params, s);
+  if (a.features <= 512)
+    return launch(what, TFT_KERNEL(norm_kernel<T, true, 1, S>), dim3((a.rows + 3) / 4), 256, params, s);
+  if (a.features <= 8192)
+    return launch(what, TFT_KERNEL(norm_kernel<T, false, 1, S>), dim3(a.rows), norm_threads(a.features, 1), params, s);
+  return launch(what, TFT_KERNEL(norm_kernel<T, false, 2, S>), dim3(a.rows), norm_threads(a.features, 2), params, s);
 }
 
+// Two workgroups a CU: more of them hide more of a row's latency and leave more partial sums
+// behind.  8192 x 4096 bf16: 512 take 43.7 us, 256 45.3, 768 50, 1024 48.
 constexpr uint32_t kNormBackGroups = 512;
 
 uint32_t norm_back_groups(int64_t rows, int64_t features) {
-  const int64_t teams = features <= 1024 ? (rows + 3) / 4 : rows;
+  const int64_t teams = features <= 512 ? (rows + 3) / 4 : rows;
   return (uint32_t)(teams < (int64_t)kNormBackGroups ? teams : (int64_t)kNormBackGroups);
 }
 
@@ -1111,12 +1191,10 @@ int launch_norm_back(const char* what, const NormBackArgs& a, hipStream_t s) {
   NormBackArgs args = a;
   void* params[] = {&args};
   const dim3 grid(norm_back_groups(a.rows, a.features));
-  if (a.features <= 512) return launch(what, TFT_KERNEL(norm_back_kernel<T, 1, 1>), grid, 256, params, s);
-  if (a.features <= 1024) return launch(what, TFT_KERNEL(norm_back_kernel<T, 1, 2>), grid, 256, params, s);
-  if (a.features <= 2048) return launch(what, TFT_KERNEL(norm_back_kernel<T, 4, 1>), grid, 256, params, s);
-  if (a.features <= 4096) return launch(what, TFT_KERNEL(norm_back_kernel<T, 4, 2>), grid, 256, params, s);
-  if (a.features <= 8192) return launch(what, TFT_KERNEL(norm_back_kernel<T, 8, 2>), grid, 512, params, s);
-  return launch(what, TFT_KERNEL(norm_back_kernel<T, 8, 4>), grid, 512, params, s);
+  if (a.features <= 512) return launch(what, TFT_KERNEL(norm_back_kernel<T, true, 1>), grid, 256, params, s);
+  if (a.features <= 8192)
+    return launch(what, TFT_KERNEL(norm_back_kernel<T, false, 1>), grid, norm_threads(a.features, 1), params, s);
+  return launch(what, TFT_KERNEL(norm_back_kernel<T, false, 2>), grid, norm_threads(a.features, 2), params, s);
 }
 
 int launch_column_reduce(const char* what, const float* partial, void* out, uint32_t groups,
@@ -1138,12 +1216,11 @@ uint32_t column_sum_groups(int64_t rows, int64_t columns) {
 
 // How a weight gradient is cut.
 struct WgradPlan {
-  int parts;         // bf16 parts of the gradient
-  bool split_first;  // they are written to the workspace
-  int64_t padded;    // row length of the parts
+  bool align_first;  // the gradient is copied to aligned rows of the workspace
+  int64_t padded;    // their length
   bool large;
-  uint32_t tiles_o, tiles_f, steps_per_part, steps, whole, cut, splits;
-  int64_t parts_bytes, partial_bytes;
+  uint32_t tiles_o, tiles_f, steps, whole, cut, splits;
+  int64_t aligned_bytes, partial_bytes;
 };
 
 constexpr int64_t kLarge = 256, kSmall = 128;  // tiles; one large or two small ones fill a CU's LDS
@@ -1152,13 +1229,12 @@ constexpr int64_t kCUs = 256;
 WgradPlan plan_wgrad(int64_t rows, int64_t out_features, int64_t features, int64_t grad_stride,
                      int dtype, bool aligned) {
   WgradPlan p{};
-  p.parts = dtype == TFT_F32 ? 3 : dtype == TFT_F16 ? 2 : 1;
-  p.split_first = dtype != TFT_BF16 || !aligned || out_features % 8 || grad_stride % 8 ||
+  p.align_first = !aligned || out_features % 8 || grad_stride % 8 ||
                   grad_stride < out_features;  // a row that stands for several (an expanded gradient)
-  p.padded = p.split_first ? (out_features + 7) / 8 * 8 : grad_stride;
-  p.parts_bytes = p.split_first ? (p.parts * rows * p.padded * 2 + 255) / 256 * 256 : 0;
-  p.steps_per_part = (uint32_t)((rows + kStep - 1) / kStep);
-  p.steps = p.steps_per_part * p.parts;
+  p.padded = p.align_first ? (out_features + 7) / 8 * 8 : grad_stride;
+  p.aligned_bytes = p.align_first ? (rows * p.padded * esize(dtype) + 255) / 256 * 256 : 0;
+  const int tokens = dtype == TFT_F32 ? Parts<F32>::kTokens : dtype == TFT_F16 ? Parts<F16>::kTokens : Parts<BF16>::kTokens;
+  p.steps = (uint32_t)((rows + tokens - 1) / tokens);
   const int64_t large_tiles = ((out_features + kLarge - 1) / kLarge) * ((features + kLarge - 1) / kLarge);
   p.large = large_tiles >= 128;
   const int64_t size = p.large ? kLarge : kSmall, at_once = p.large ? kCUs : 2 * kCUs;
@@ -1176,6 +1252,29 @@ WgradPlan plan_wgrad(int64_t rows, int64_t out_features, int64_t features, int64
   p.splits = (uint32_t)splits;
   p.partial_bytes = splits * cut * size * size * 4;
   return p;
+}
+
+template <typename T>
+int launch_wgrad(const char* what, const WgradArgs& a, const WgradPlan& p, const AlignArgs& align, hipStream_t s) {
+  if (p.align_first && a.rows > 0) {
+    AlignArgs args = align;
+    void* params[] = {&args};
+    const uint64_t groups = (align.chunks + 255) / 256;
+    if (int rc = launch(what, TFT_KERNEL(align_kernel<T>), dim3((uint32_t)(groups < 16384 ? groups : 16384)), 256,
+                        params, s))
+      return rc;
+  }
+  WgradArgs args = a;
+  void* params[] = {&args};
+  const dim3 grid(p.whole + p.cut * p.splits);
+  if (int rc = p.large ? launch(what, TFT_KERNEL(wgrad_kernel<T, kLarge, kLarge, 2, 4>), grid, 512, params, s)
+                       : launch(what, TFT_KERNEL(wgrad_kernel<T, kSmall, kSmall, 2, 2>), grid, 256, params, s))
+    return rc;
+  if (!p.cut) return TFT_OK;
+  const int64_t size = p.large ? kLarge : kSmall;
+  const dim3 join((uint32_t)(p.cut * (size * size / 1024)));
+  return p.large ? launch(what, TFT_KERNEL(wgrad_join_kernel<kLarge, kLarge>), join, 256, params, s)
+                 : launch(what, TFT_KERNEL(wgrad_join_kernel<kSmall, kSmall>), join, 256, params, s);
 }
 
 }  // namespace
@@ -1196,9 +1295,10 @@ int tft_pack_e4m3(void* values, void* exponents, const void* x, int64_t rows, in
              pitch, (uint32_t)(rows * per_row), make_divider(per_row)};
   void* params[] = {&a};
   const dim3 grid((a.blocks + kPackBlocks - 1) / kPackBlocks);
-  const void* k = dtype == TFT_F32 ? TFT_KERNEL(pack_kernel<F32>)
-                  : dtype == TFT_BF16 ? TFT_KERNEL(pack_kernel<BF16>)
-                                      : TFT_KERNEL(pack_kernel<F16>);
+  const bool far = rows * features * (esize(dtype) + 1) >= kLastLevelCache;
+#define TFT_PACK(T) (far ? TFT_KERNEL(pack_kernel<T, true>) : TFT_KERNEL(pack_kernel<T, false>))
+  const void* k = dtype == TFT_F32 ? TFT_PACK(F32) : dtype == TFT_BF16 ? TFT_PACK(BF16) : TFT_PACK(F16);
+#undef TFT_PACK
   return launch(what, k, grid, kPackThreads, params, static_cast<hipStream_t>(stream));
 }
 
@@ -1217,14 +1317,17 @@ int tft_unpack_e4m3(void* out, const void* values, const void* exponents, const 
   UnpackArgs a{out, static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents), column_scale,
                features, pitch, (uint32_t)(rows * per_row), make_divider(per_row)};
   void* params[] = {&a};
-  const dim3 grid((a.blocks + kPackBlocks - 1) / kPackBlocks);
+  const dim3 grid((a.blocks + kUnpackBlocks - 1) / kUnpackBlocks);
   const int st = column_scale ? scale_dtype : TFT_F32;
-#define TFT_UNPACK(T)                                                     \
-  (st == TFT_F32 ? TFT_KERNEL(unpack_kernel<T, F32>)                      \
-   : st == TFT_BF16 ? TFT_KERNEL(unpack_kernel<T, BF16>)                  \
-                    : TFT_KERNEL(unpack_kernel<T, F16>))
+  const bool far = rows * features * (esize(dtype) + 1) >= kLastLevelCache;
+#define TFT_UNPACK2(T, W) (far ? TFT_KERNEL(unpack_kernel<T, W, true>) : TFT_KERNEL(unpack_kernel<T, W, false>))
+#define TFT_UNPACK(T)                                   \
+  (st == TFT_F32 ? TFT_UNPACK2(T, F32)                  \
+   : st == TFT_BF16 ? TFT_UNPACK2(T, BF16)              \
+                    : TFT_UNPACK2(T, F16))
   const void* k = dtype == TFT_F32 ? TFT_UNPACK(F32) : dtype == TFT_BF16 ? TFT_UNPACK(BF16) : TFT_UNPACK(F16);
 #undef TFT_UNPACK
+#undef TFT_UNPACK2
   return launch(what, k, grid, kPackThreads, params, static_cast<hipStream_t>(stream));
 }
 
@@ -1258,9 +1361,10 @@ int tft_rms_norm(void* y, void* h, void* values, void* exponents, float* rstd, c
              (uint32_t)rows, (int)features, x_row_stride, residual_row_stride, pitch,
              weight_dtype == TFT_F32 ? 1 : 0, eps};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == TFT_F32) return launch_norm<F32>(what, a, s);
-  if (dtype == TFT_BF16) return launch_norm<BF16>(what, a, s);
-  return launch_norm<F16>(what, a, s);
+  const bool far = rows * features * (esize(dtype) * (residual ? 4 : 2) + (values ? 1 : 0)) >= kLastLevelCache;
+#define TFT_NORM(T) (far ? launch_norm<T, true>(what, a, s) : launch_norm<T, false>(what, a, s))
+  return dtype == TFT_F32 ? TFT_NORM(F32) : dtype == TFT_BF16 ? TFT_NORM(BF16) : TFT_NORM(F16);
+#undef TFT_NORM
 }
 
 int64_t tft_rms_norm_backward_workspace(int64_t rows, int64_t features) {
@@ -1303,10 +1407,9 @@ int tft_rms_norm_backward(void* grad_x, void* grad_weight, void* workspace, int6
   NormBackArgs a{grad_y, grad_h, static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents), rstd,
                  weight, grad_x, partial, (uint32_t)rows, (int)features, grad_y_row_stride, grad_h_row_stride,
                  pitch, weight_dtype == TFT_F32 ? 1 : 0};
-  int rc;
-  if (dtype == TFT_F32) rc = launch_norm_back<F32>(what, a, s);
-  else if (dtype == TFT_BF16) rc = launch_norm_back<BF16>(what, a, s);
-  else rc = launch_norm_back<F16>(what, a, s);
+  const int rc = dtype == TFT_F32    ? launch_norm_back<F32>(what, a, s)
+                 : dtype == TFT_BF16 ? launch_norm_back<BF16>(what, a, s)
+                                     : launch_norm_back<F16>(what, a, s);
   if (rc || !grad_weight) return rc;
   return launch_column_reduce(what, partial, grad_weight, norm_back_groups(rows, features), features,
                               weight_dtype, s);
@@ -1350,7 +1453,7 @@ int64_t tft_linear_weight_grad_workspace(const void* grad_out, int64_t rows, int
   if (rows <= 0 || out_features <= 0 || features <= 0) return 0;
   const WgradPlan p = plan_wgrad(rows, out_features, features, grad_row_stride, dtype,
                                  (reinterpret_cast<uintptr_t>(grad_out) & 15u) == 0);
-  return p.parts_bytes + p.partial_bytes;
+  return p.aligned_bytes + p.partial_bytes;
 }
 
 int tft_linear_weight_grad(void* grad_weight, void* workspace, int64_t workspace_bytes,
@@ -1378,45 +1481,26 @@ int tft_linear_weight_grad(void* grad_weight, void* workspace, int64_t workspace
   const WgradPlan p = plan_wgrad(rows, out_features, features, grad_row_stride, dtype,
                                  (reinterpret_cast<uintptr_t>(grad_out) & 15u) == 0);
   // offsets within a step's rows are 31 bits
-  if (p.padded * 2 * kStep >= (1ll << 31) || pitch * kStep >= (1ll << 31))
+  if (p.padded * esize(dtype) * 64 >= (1ll << 31) || pitch * 64 >= (1ll << 31))
     return fail(TFT_ERR_UNSUPPORTED, "%s: rows of %lld gradients or %lld packed values are too long", what,
                 (long long)p.padded, (long long)pitch);
-  if ((int64_t)p.steps_per_part * p.parts >= (1ll << 31) ||
-      (int64_t)p.tiles_o * p.tiles_f * 4 >= (1ll << 31))
+  if ((int64_t)p.tiles_o * p.tiles_f * 4 >= (1ll << 31))
     return fail(TFT_ERR_UNSUPPORTED, "%s: too many tiles for one grid", what);
-  const int64_t needed = p.parts_bytes + p.partial_bytes;
+  const int64_t needed = p.aligned_bytes + p.partial_bytes;
   if (needed && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < needed))
     return fail(TFT_ERR_INVALID_ARGUMENT, "%s: workspace of %lld bytes, %lld are needed", what,
                 (long long)workspace_bytes, (long long)needed);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const uint16_t* d = static_cast<const uint16_t*>(grad_out);
-  if (p.split_first && rows > 0) {
-    SplitArgs a{grad_out, static_cast<uint16_t*>(workspace), rows, out_features, grad_row_stride, p.padded,
-                (uint64_t)rows * (p.padded / 8)};
-    void* params[] = {&a};
-    const uint64_t groups = (a.chunks + 255) / 256;
-    const dim3 grid((uint32_t)(groups < 16384 ? groups : 16384));
-    const void* k = dtype == TFT_F32 ? TFT_KERNEL(split_kernel<F32, 3>)
-                    : dtype == TFT_BF16 ? TFT_KERNEL(split_kernel<BF16, 1>)
-                                        : TFT_KERNEL(split_kernel<F16, 2>);
-    if (int rc = launch(what, k, grid, 256, params, s)) return rc;
-    d = a.parts;
-  }
-  WgradArgs a{d, static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents), column_scale,
-              grad_weight, reinterpret_cast<float*>(static_cast<char*>(workspace) + p.parts_bytes), rows,
-              p.padded, pitch, (uint32_t)out_features, (uint32_t)features,
-              (uint32_t)((features + kBlock - 1) / kBlock), p.tiles_o, p.tiles_f, p.whole, p.cut, p.splits,
-              p.steps_per_part, p.steps, scale_dtype, out_dtype};
-  void* params[] = {&a};
-  const dim3 grid(p.whole + p.cut * p.splits);
-  if (int rc = p.large ? launch(what, TFT_KERNEL(wgrad_kernel<kLarge, kLarge, 2, 4>), grid, 512, params, s)
-                       : launch(what, TFT_KERNEL(wgrad_kernel<kSmall, kSmall, 2, 2>), grid, 256, params, s))
-    return rc;
-  if (!p.cut) return TFT_OK;
-  const int64_t size = p.large ? kLarge : kSmall;
-  const dim3 join((uint32_t)(p.cut * (size * size / 1024)));
-  return p.large ? launch(what, TFT_KERNEL(wgrad_join_kernel<kLarge, kLarge>), join, 256, params, s)
-                 : launch(what, TFT_KERNEL(wgrad_join_kernel<kSmall, kSmall>), join, 256, params, s);
+  const AlignArgs align{grad_out, workspace, out_features, grad_row_stride, p.padded,
+                        (uint64_t)rows * (uint64_t)(p.padded / 8)};
+  const WgradArgs a{p.align_first ? workspace : grad_out, static_cast<const uint8_t*>(values),
+                    static_cast<const uint8_t*>(exponents), column_scale, grad_weight,
+                    reinterpret_cast<float*>(static_cast<char*>(workspace) + p.aligned_bytes), rows, p.padded, pitch,
+                    (uint32_t)out_features, (uint32_t)features, (uint32_t)((features + kBlock - 1) / kBlock),
+                    p.tiles_o, p.tiles_f, p.whole, p.cut, p.splits, p.steps, scale_dtype, out_dtype};
+  if (dtype == TFT_F32) return launch_wgrad<F32>(what, a, p, align, s);
+  if (dtype == TFT_BF16) return launch_wgrad<BF16>(what, a, p, align, s);
+  return launch_wgrad<F16>(what, a, p, align, s);
 }
 
 }  // extern "C"
