@@ -255,10 +255,10 @@ def test_c_entries_refuse_without_a_gpu():
     assert space(at, 64, 63, 130, 63, 144, 1) == 64 * 64 * 2
     assert space(at, 64, 64, 130, 0, 144, 1) == 64 * 64 * 2  # one row that stands for all
     assert space(at, 0, 64, 130, 64, 144, 1) == 0
-    # 3 x 2 tiles of 128, cut along 320 tokens into pieces of four steps: one piece
-    assert space(at, 320, 384, 256, 384, 256, 1) == 0
-    # along 640 tokens: two pieces of six tiles in fp32
-    assert space(at, 640, 384, 256, 384, 256, 1) == 2 * 6 * 128 * 128 * 4
+    # one small tile and 16 tokens: nothing to cut; 4096 tokens: pieces, in fp32
+    assert space(at, 16, 128, 128, 128, 128, 1) == 0
+    assert space(at, 4096, 128, 128, 128, 128, 1) % (128 * 128 * 4) == 0
+    assert space(at, 4096, 128, 128, 128, 128, 1) >= 2 * 128 * 128 * 4
 
 
 # --- modules ------------------------------------------------------------------------------------

@@ -1226,6 +1226,26 @@ struct WgradPlan {
 constexpr int64_t kLarge = 256, kSmall = 128;  // tiles; one large or two small ones fill a CU's LDS
 constexpr int64_t kCUs = 256;
 
+// Microseconds that the tiles of one size take with those left over from whole rounds of the chip
+// cut into `splits` pieces along the tokens.  A step of 16 x kProducts tokens takes 0.8 us of a
+// small tile alone on its CU, 1.15 of two beside each other and 1.8 of a large one; a round of
+// workgroups starts and ends in 7; partial tiles are written and read at 7 TB/s and joined by a
+// launch of 2.
+double wgrad_time(bool large, int64_t tiles, int64_t steps, int products, int64_t splits) {
+  const int64_t at_once = large ? kCUs : 2 * kCUs, size = large ? kLarge : kSmall, pieces = tiles % at_once * splits;
+  const double step = products / 4.0;
+  const double whole = (double)(tiles / at_once) * (3.0 + steps * step * (large ? 1.8 : 1.15));
+  if (!pieces) return whole;
+  const double each = step * (large ? 1.8 : pieces > kCUs ? 1.15 : 0.8);
+  const int64_t rounds = (pieces + at_once - 1) / at_once, longest = (steps + splits - 1) / splits;
+  return whole + rounds * (7.0 + longest * each) + (splits > 1 ? 2.0 + pieces * size * size * 8 / 7e6 : 0.0);
+}
+
+// Large tiles read LDS less per product and small ones fill the chip with less; which of them, and
+// how many pieces, is the least of the times above.  Measured, us, large tiles in their best number
+// of pieces / small ones: 8192 tokens, 4096 x 4096 bf16 242 (1) / 313 (1); 8192, 1024 x 4096
+// 82 (4) / 90 (2); 4096, 2048 x 2048 fp16 78 (4) / 91 (2); 1024, 768 x 768 bf16 21 (5) / 15 (3);
+// 1000, 1001 x 768 fp32 31 (10) / 28 (3).
 WgradPlan plan_wgrad(int64_t rows, int64_t out_features, int64_t features, int64_t grad_stride,
                      int dtype, bool aligned) {
   WgradPlan p{};
@@ -1234,23 +1254,27 @@ WgradPlan plan_wgrad(int64_t rows, int64_t out_features, int64_t features, int64
   p.padded = p.align_first ? (out_features + 7) / 8 * 8 : grad_stride;
   p.aligned_bytes = p.align_first ? (rows * p.padded * esize(dtype) + 255) / 256 * 256 : 0;
   const int tokens = dtype == TFT_F32 ? Parts<F32>::kTokens : dtype == TFT_F16 ? Parts<F16>::kTokens : Parts<BF16>::kTokens;
+  const int parts = dtype == TFT_F32 ? Parts<F32>::kParts : dtype == TFT_F16 ? Parts<F16>::kParts : Parts<BF16>::kParts;
   p.steps = (uint32_t)((rows + tokens - 1) / tokens);
-  const int64_t large_tiles = ((out_features + kLarge - 1) / kLarge) * ((features + kLarge - 1) / kLarge);
-  p.large = large_tiles >= 128;
-  const int64_t size = p.large ? kLarge : kSmall, at_once = p.large ? kCUs : 2 * kCUs;
-  p.tiles_o = (uint32_t)((out_features + size - 1) / size);
-  p.tiles_f = (uint32_t)((features + size - 1) / size);
-  // whole rounds of the chip take one workgroup per tile; what is left over is cut along the
-  // tokens until it fills the chip too, in pieces of at least four steps
-  const int64_t tiles = (int64_t)p.tiles_o * p.tiles_f;
-  int64_t cut = tiles % at_once, splits = cut ? at_once / cut : 1;
-  const int64_t most = p.steps / 4 > 1 ? p.steps / 4 : 1;
-  if (splits > most) splits = most;
-  if (splits == 1) cut = 0;
-  p.whole = (uint32_t)(tiles - cut);
-  p.cut = (uint32_t)cut;
-  p.splits = (uint32_t)splits;
-  p.partial_bytes = splits * cut * size * size * 4;
+  double best = 0.0;
+  for (int large = 1; large >= 0; --large) {
+    const int64_t size = large ? kLarge : kSmall, at_once = large ? kCUs : 2 * kCUs;
+    const int64_t across = (out_features + size - 1) / size, along = (features + size - 1) / size;
+    const int64_t tiles = across * along, over = tiles % at_once;
+    const int64_t most = over == 0 ? 1 : at_once / over < p.steps ? at_once / over : p.steps > 1 ? p.steps : 1;
+    for (int64_t splits = 1; splits <= most; ++splits) {
+      const double time = wgrad_time(large, tiles, p.steps, tokens / 16 * parts, splits);
+      if (best != 0.0 && time >= best) continue;
+      best = time;
+      p.large = large;
+      p.tiles_o = (uint32_t)across;
+      p.tiles_f = (uint32_t)along;
+      p.splits = (uint32_t)splits;
+      p.cut = (uint32_t)(splits > 1 ? over : 0);
+      p.whole = (uint32_t)(tiles - p.cut);
+      p.partial_bytes = p.cut * splits * size * size * 4;
+    }
+  }
   return p;
 }
 
