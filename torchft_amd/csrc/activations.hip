@@ -871,9 +871,13 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
   constexpr int kXChunks = kTokens * F / 16 / kThreads;  // 16-byte chunks of X
   constexpr int kDTile = kParts * kTokens * O, kXTile = kTokens * F;
   constexpr int kFragO = O / WO / 32, kFragF = F / WF / 32;
-  __shared__ __attribute__((aligned(128))) uint16_t lds[2 * (kDTile + kXTile)];
-  uint16_t* const lds_d = lds;               // two tiles, [part][token][O]
-  uint16_t* const lds_x = lds + 2 * kDTile;  // two tiles, [token][F]
+  // bf16 goes from memory into LDS by itself, past the registers (kDirect), into one of three buffers
+  // because a tile is asked for while two are in use; what has to be split goes through registers
+  constexpr bool kDirect = kParts == 1;
+  constexpr int kDBuffers = kDirect ? 3 : 2;
+  __shared__ __attribute__((aligned(128))) uint16_t lds[kDBuffers * kDTile + 2 * kXTile];
+  uint16_t* const lds_d = lds;                       // tiles [part][token][O]
+  uint16_t* const lds_x = lds + kDBuffers * kDTile;  // two tiles [token][F]
 
   const bool is_cut = blockIdx.x >= a.whole;
   uint32_t tile_o, tile_f, slot = 0, step_begin = 0, step_end = a.steps;
@@ -893,10 +897,13 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
 #pragma unroll
   for (int i = 0; i < kDChunks; ++i) {
     const int c = i * kThreads + threadIdx.x, t = c / (O / 8), j = c % (O / 8);
-    d_off[i] = o0 + j * 8 < a.out_features ? (uint32_t)((t * a.d_stride + j * 8) * sizeof(elem_t)) : 0x80000000u;
-    d_lds[i] = t * O + (((j >> 1) ^ spread(t)) << 4) + ((j & 1) << 3);
+    const int spread_j = (((j >> 1) ^ spread(t)) << 1) + (j & 1);
+    // direct loads lie in LDS in the order of the lanes, so a lane asks for the chunk whose place is its own
+    const int from = kDirect ? spread_j : j;
+    d_off[i] = o0 + from * 8 < a.out_features ? (uint32_t)((t * a.d_stride + from * 8) * sizeof(elem_t)) : 0x80000000u;
+    d_lds[i] = t * O + spread_j * 8;
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int swap = (lane >> 2) & 1;  // lanes 4 .. 7 of eight write a unit's halves the other way round
 #pragma unroll
   for (int i = 0; i < kXChunks; ++i) {
@@ -943,6 +950,22 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
       x_reg[i] = __builtin_amdgcn_raw_buffer_load_b128(x, x_off[i], 0, 0);
       e_reg[i] = __builtin_amdgcn_raw_buffer_load_b8(e, e_off[i], 0, 0);
     }
+  };
+  // D past the registers, into buffer `to`.  The compiler does not know of these loads: who reads
+  // the buffer has waited for them by hand.
+  auto fetch_d_direct = [&](int to) {
+    const uint64_t base = (uint64_t)d_at;
+    const int64_t bytes = (left * a.d_stride - o0) * (int64_t)sizeof(elem_t);
+    const u32x4 d = {(uint32_t)base, (uint32_t)(base >> 32) & 0xffffu,
+                     (uint32_t)max((int64_t)0, min(bytes, (int64_t)0x7fffffff)), 0x00020000u};
+    const uint32_t at =
+        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)(lds_d + to * kDTile + wave * 512);
+#pragma unroll
+    for (int i = 0; i < kDChunks; ++i)  // 64 lanes of 16 bytes, one behind the other, from M0 on
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                   :
+                   : "v"(d_off[i]), "s"(d), "s"(at + i * kThreads * 16)
+                   : "memory");
   };
   auto advance = [&]() {
     left -= kTokens;
@@ -999,15 +1022,15 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
   // A step's products: kTokens / 16 groups of tokens, every part of D with the same X
   constexpr int kProducts = kTokens / 16 * kParts;
   bf16x8 d[2][kFragO], x[2][kFragF];
-  auto load = [&](int product, int buf) {
+  auto load = [&](int product, int d_buf, int x_buf) {
     const int group = product / kParts, part = product % kParts;
     if (part == 0)
 #pragma unroll
       for (int i = 0; i < kFragF; ++i)
-        x[group & 1][i] = operand(&lds_x[buf * kXTile + x_read[i] + group * 16 * F], F);
+        x[group & 1][i] = operand(&lds_x[x_buf * kXTile + x_read[i] + group * 16 * F], F);
 #pragma unroll
     for (int j = 0; j < kFragO; ++j)
-      d[product & 1][j] = operand(&lds_d[buf * kDTile + d_read[j] + (part * kTokens + group * 16) * O], O);
+      d[product & 1][j] = operand(&lds_d[d_buf * kDTile + d_read[j] + (part * kTokens + group * 16) * O], O);
   };
   auto multiply = [&](int product) {
 #pragma unroll
@@ -1019,40 +1042,58 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
   };
 
   // While one product runs, the next one's operands come out of LDS; meanwhile the next step's
-  // tile goes into the other buffer, and the tile after that is asked for.  One barrier a step:
+  // tile goes into another buffer, and the tile after that is asked for.  One barrier a step:
   // behind it the next tile is whole, and nobody reads the present one any more.
   static_assert(kProducts % 2 == 0 && kTokens / 16 % 2 == 0, "the operands' turns close with a step");
   if (step_begin < step_end) {
-    fetch_d();
+    int d_now = 0, d_next = 1, d_after = kDirect ? 2 : 0, x_now = 0;
+    if constexpr (kDirect) fetch_d_direct(0);
+    else fetch_d();
     fetch_x();
     advance();
-    stage_d(0);
+    if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    else stage_d(0);
     stage_x(0);
-    fetch_d();
+    if constexpr (kDirect) fetch_d_direct(1);
+    else fetch_d();
     fetch_x();
     advance();
     __syncthreads();
-    load(0, 0);
-    int buf = 0;
-    for (uint32_t s = step_begin; s < step_end; ++s, buf ^= 1) {
+    load(0, 0, 0);
+    for (uint32_t s = step_begin; s < step_end; ++s) {
 #pragma unroll
       for (int k = 0; k + 1 < kProducts; ++k) {
-        load(k + 1, buf);
-        if (k == 1) {
-          stage_d(buf ^ 1);
+        load(k + 1, d_now, x_now);
+        if (kDirect && k == 1) {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the next step's D and X, asked for a step ago
+          fetch_d_direct(d_after);
+          stage_x(x_now ^ 1);
+          fetch_x();
+          advance();
+        }
+        if (!kDirect && k == 1) {
+          stage_d(d_next);
           fetch_d();
         }
-        if (k == 2) {
-          stage_x(buf ^ 1);
+        if (!kDirect && k == 2) {
+          stage_x(x_now ^ 1);
           fetch_x();
           advance();
         }
         multiply(k);
       }
-      __syncthreads();
-      load(0, buf ^ 1);
+      // waits for this wavefront's LDS accesses, not for the loads under way
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      load(0, d_next, x_now ^ 1);
       multiply(kProducts - 1);
+      x_now ^= 1;
+      const int before = d_now;
+      d_now = d_next;
+      d_next = d_after;
+      d_after = before;
+      if (!kDirect) d_next = before, d_after = d_now;
     }
+    if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing lands in LDS any more
   }
 
   // Of 32 features x 32 output rows a lane holds output row lane % 32, features 8q + 4 (lane / 32)
