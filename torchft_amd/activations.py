@@ -21,6 +21,7 @@ device, never synchronise, and have no CPU path.  The reference has no counterpa
 
 from __future__ import annotations
 
+import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -76,7 +77,8 @@ def _require_gpu(t: torch.Tensor, what: str) -> None:
 
 
 def _require_same_device(t: torch.Tensor, device: torch.device, what: str) -> None:
-    _require_gpu(t, what)
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        _require_gpu(t, what)
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, expected {device}")
 
@@ -88,10 +90,7 @@ def _matrix(x: torch.Tensor, what: str) -> Tuple[int, int, int]:
         raise ValueError(f"{what}: a scalar has no rows")
     features = x.shape[-1]
     if features == 0 or x.numel() == 0:
-        rows = 1
-        for n in x.shape[:-1]:
-            rows *= n
-        return rows, features, features
+        return math.prod(x.shape[:-1]), features, features
     if features > 1 and x.stride(-1) != 1:
         raise ValueError(f"{what}: the elements of a row must be consecutive, strides are {x.stride()}")
     if x.dim() == 2 and x.shape[0] > 1:
@@ -115,6 +114,12 @@ def _as_rows(x: torch.Tensor) -> torch.Tensor:
     except ValueError:
         return x.contiguous()
     return x
+
+
+def _contiguous_like(x: torch.Tensor) -> torch.Tensor:
+    if x.is_contiguous():
+        return torch.empty_like(x, requires_grad=False)
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _pitch(features: int) -> int:
@@ -154,38 +159,37 @@ class PackedActivation:
         shape: Optional[Tuple[int, ...]] = None,
         dtype: Optional[torch.dtype] = None,
     ) -> None:
-        what = "PackedActivation"
-        _require_gpu(values, f"{what}: values")
-        _require_same_device(exponents, values.device, f"{what}: exponents")
+        _require_gpu(values, "PackedActivation: values")
+        device = values.device
+        _require_same_device(exponents, device, "PackedActivation: exponents")
         if values.dtype not in (torch.float8_e4m3fn, torch.uint8) or exponents.dtype != torch.uint8:
-            raise TypeError(f"{what}: expected float8_e4m3fn (or uint8) values and uint8 exponents, "
-                            f"got {values.dtype} and {exponents.dtype}")
+            raise TypeError("PackedActivation: expected float8_e4m3fn (or uint8) values and uint8 "
+                            f"exponents, got {values.dtype} and {exponents.dtype}")
         if features < 0 or values.dim() != 2 or values.shape[1] != _pitch(features) \
                 or not values.is_contiguous():
-            raise ValueError(f"{what}: values must be contiguous [rows, {_pitch(features)}] for "
+            raise ValueError(f"PackedActivation: values must be contiguous [rows, {_pitch(features)}] for "
                              f"{features} features, got {tuple(values.shape)}")
-        if tuple(exponents.shape) != (values.shape[0], _blocks(features)) or not exponents.is_contiguous():
-            raise ValueError(f"{what}: exponents must be contiguous "
-                             f"{(values.shape[0], _blocks(features))}, got {tuple(exponents.shape)}")
+        rows = values.shape[0]
+        if exponents.shape != (rows, _blocks(features)) or not exponents.is_contiguous():
+            raise ValueError(f"PackedActivation: exponents must be contiguous "
+                             f"{(rows, _blocks(features))}, got {tuple(exponents.shape)}")
         if values.data_ptr() % 16:
-            raise ValueError(f"{what}: values must start at a multiple of 16 bytes")
-        _vector(column_scale, features, values.device, f"{what}: column_scale")
+            raise ValueError("PackedActivation: values must start at a multiple of 16 bytes")
+        _vector(column_scale, features, device, "PackedActivation: column_scale")
         if shape is None:
-            shape = (values.shape[0], features)
+            shape = (rows, features)
         else:
-            rows = 1
-            for n in shape[:-1]:
-                rows *= n
-            if not shape or shape[-1] != features or rows != values.shape[0]:
-                raise ValueError(f"{what}: shape {tuple(shape)} does not hold {values.shape[0]} rows "
-                                 f"of {features} features")
+            shape = tuple(shape)
+            if not shape or shape[-1] != features or math.prod(shape[:-1]) != rows:
+                raise ValueError(f"PackedActivation: shape {shape} does not hold {rows} rows of "
+                                 f"{features} features")
         if dtype is None:
             dtype = torch.bfloat16 if column_scale is None else column_scale.dtype
-        _dtype_code(dtype, what)
+        _dtype_code(dtype, "PackedActivation")
         self.values = values
         self.exponents = exponents
         self.features = features
-        self.shape = tuple(shape)
+        self.shape = shape
         self.dtype = dtype
         self.column_scale = column_scale
 
@@ -262,32 +266,31 @@ def rms_norm_forward(
     residual), rstd = 1 / sqrt(mean(h^2) + eps) in fp32 of [rows], y = h * rstd * weight, and the
     normalised rows h * rstd packed with ``weight`` as their column scale.  ``eps=None`` is the
     type's machine epsilon, as in ``torch.nn.RMSNorm``.  No autograd: see :func:`rms_norm`."""
-    what = "rms_norm"
-    rows, features, stride = _matrix(x, f"{what}: x")
-    code = _dtype_code(x.dtype, what)
-    device = x.device
+    rows, features, stride = _matrix(x, "rms_norm: x")
+    dtype, device = x.dtype, x.device
+    code = _dtype_code(dtype, "rms_norm")
     if features > MAX_NORM_FEATURES:
-        raise ValueError(f"{what}: {features} features, at most {MAX_NORM_FEATURES}")
-    _vector(weight, features, device, f"{what}: weight")
-    _check_norm_weight(weight, x.dtype, what)
+        raise ValueError(f"rms_norm: {features} features, at most {MAX_NORM_FEATURES}")
+    _vector(weight, features, device, "rms_norm: weight")
+    _check_norm_weight(weight, dtype, "rms_norm")
     if eps is None:
-        eps = torch.finfo(x.dtype).eps
+        eps = torch.finfo(dtype).eps
     if not eps >= 0.0:
-        raise ValueError(f"{what}: eps must be at least 0, got {eps}")
+        raise ValueError(f"rms_norm: eps must be at least 0, got {eps}")
     residual_stride = 0
     if residual is not None:
-        _require_same_device(residual, device, f"{what}: residual")
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise ValueError(f"{what}: residual is {residual.dtype}{list(residual.shape)}, "
-                             f"x is {x.dtype}{list(x.shape)}")
-        _, _, residual_stride = _matrix(residual, f"{what}: residual")
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=device)
+        _require_same_device(residual, device, "rms_norm: residual")
+        if residual.shape != x.shape or residual.dtype != dtype:
+            raise ValueError(f"rms_norm: residual is {residual.dtype}{list(residual.shape)}, "
+                             f"x is {dtype}{list(x.shape)}")
+        _, _, residual_stride = _matrix(residual, "rms_norm: residual")
+    y = _contiguous_like(x)
+    h = x if residual is None else _contiguous_like(x)
     rstd = torch.empty(rows, dtype=torch.float32, device=device)
     values = exponents = packed = None
     if pack:
         values, exponents = _buffers(rows, features, device)
-        packed = _trusted(values, exponents, features, weight, tuple(x.shape), x.dtype)
+        packed = _trusted(values, exponents, features, weight, tuple(x.shape), dtype)
     _launch(
         "tft_rms_norm", device, y.data_ptr(), None if residual is None else h.data_ptr(),
         values.data_ptr() if pack else None, exponents.data_ptr() if pack else None,
@@ -308,29 +311,28 @@ def rms_norm_backward(
     """(grad_x, grad_weight) of :func:`rms_norm_forward` from what it packed.  ``grad_h`` is the
     gradient that reaches h from its other readers; ``grad_x`` is the residual's gradient too.
     ``grad_weight`` has the weight's type and is None where there is no weight."""
-    what = "rms_norm_backward"
-    rows, features, stride = _matrix(grad_y, f"{what}: grad_y")
-    code = _dtype_code(grad_y.dtype, what)
-    device = grad_y.device
+    rows, features, stride = _matrix(grad_y, "rms_norm_backward: grad_y")
+    dtype, device = grad_y.dtype, grad_y.device
+    code = _dtype_code(dtype, "rms_norm_backward")
     weight = packed.column_scale
     if (rows, features) != (packed.rows, packed.features):
-        raise ValueError(f"{what}: grad_y has {rows} rows of {features}, packed {packed.rows} rows of "
-                         f"{packed.features}")
+        raise ValueError(f"rms_norm_backward: grad_y has {rows} rows of {features}, packed {packed.rows} "
+                         f"rows of {packed.features}")
     if features > MAX_NORM_FEATURES:
-        raise ValueError(f"{what}: {features} features, at most {MAX_NORM_FEATURES}")
-    _require_same_device(packed.values, device, f"{what}: packed")
-    _check_norm_weight(weight, grad_y.dtype, what)
-    _require_same_device(rstd, device, f"{what}: rstd")
+        raise ValueError(f"rms_norm_backward: {features} features, at most {MAX_NORM_FEATURES}")
+    _require_same_device(packed.values, device, "rms_norm_backward: packed")
+    _check_norm_weight(weight, dtype, "rms_norm_backward")
+    _require_same_device(rstd, device, "rms_norm_backward: rstd")
     if rstd.dtype != torch.float32 or rstd.numel() != rows or not rstd.is_contiguous():
-        raise ValueError(f"{what}: rstd must be {rows} consecutive float32 numbers")
+        raise ValueError(f"rms_norm_backward: rstd must be {rows} consecutive float32 numbers")
     grad_h_stride = 0
     if grad_h is not None:
-        _require_same_device(grad_h, device, f"{what}: grad_h")
-        if grad_h.shape != grad_y.shape or grad_h.dtype != grad_y.dtype:
-            raise ValueError(f"{what}: grad_h is {grad_h.dtype}{list(grad_h.shape)}, grad_y is "
-                             f"{grad_y.dtype}{list(grad_y.shape)}")
-        _, _, grad_h_stride = _matrix(grad_h, f"{what}: grad_h")
-    grad_x = torch.empty(grad_y.shape, dtype=grad_y.dtype, device=device)
+        _require_same_device(grad_h, device, "rms_norm_backward: grad_h")
+        if grad_h.shape != grad_y.shape or grad_h.dtype != dtype:
+            raise ValueError(f"rms_norm_backward: grad_h is {grad_h.dtype}{list(grad_h.shape)}, grad_y is "
+                             f"{dtype}{list(grad_y.shape)}")
+        _, _, grad_h_stride = _matrix(grad_h, "rms_norm_backward: grad_h")
+    grad_x = _contiguous_like(grad_y)
     grad_weight = workspace = None
     need = 0
     if weight is not None and weight_grad:
@@ -355,15 +357,14 @@ def linear_weight_grad(
     """grad_out^T . packed of [out_features, features]: a linear layer's weight gradient from its
     packed input.  Sums are held in fp32 and rounded once to ``dtype`` (grad_out's by default);
     fp16 and fp32 gradients lose no bits."""
-    what = "linear_weight_grad"
-    rows, out_features, stride = _matrix(grad_out, f"{what}: grad_out")
-    code = _dtype_code(grad_out.dtype, what)
+    rows, out_features, stride = _matrix(grad_out, "linear_weight_grad: grad_out")
+    code = _dtype_code(grad_out.dtype, "linear_weight_grad")
     dtype = grad_out.dtype if dtype is None else dtype
-    out_code = _dtype_code(dtype, what)
+    out_code = _dtype_code(dtype, "linear_weight_grad")
     device = grad_out.device
     if rows != packed.rows:
-        raise ValueError(f"{what}: grad_out has {rows} rows, packed {packed.rows}")
-    _require_same_device(packed.values, device, f"{what}: packed")
+        raise ValueError(f"linear_weight_grad: grad_out has {rows} rows, packed {packed.rows}")
+    _require_same_device(packed.values, device, "linear_weight_grad: packed")
     scale = packed.column_scale
     features, pitch = packed.features, packed.values.shape[1]
     out = torch.empty(out_features, features, dtype=dtype, device=device)
@@ -384,16 +385,15 @@ def linear_weight_grad(
 def column_sum(x: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """The sum of x's rows in fp32, rounded once to ``dtype`` (x's by default): a bias's gradient.
     Rows are added in a fixed order."""
-    what = "column_sum"
-    rows, columns, stride = _matrix(x, what)
-    code = _dtype_code(x.dtype, what)
+    rows, columns, stride = _matrix(x, "column_sum")
+    code = _dtype_code(x.dtype, "column_sum")
     dtype = x.dtype if dtype is None else dtype
     out = torch.empty(columns, dtype=dtype, device=x.device)
     need = _native.lib().tft_column_sum_workspace(rows, columns)
     workspace = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _launch(
         "tft_column_sum", x.device, out.data_ptr(), None if workspace is None else workspace.data_ptr(),
-        need, x.data_ptr(), rows, columns, stride, _dtype_code(dtype, what), code,
+        need, x.data_ptr(), rows, columns, stride, _dtype_code(dtype, "column_sum"), code,
     )
     return out
 
@@ -497,19 +497,18 @@ def linear(
     """``torch.nn.functional.linear`` that keeps its input in 8 bits.  ``packed`` is x in that form
     where the caller has it (:func:`rms_norm`, or another layer's :func:`pack` of the same x);
     otherwise x is packed here, unless the weight needs no gradient."""
-    what = "linear"
-    _require_gpu(x, f"{what}: x")
+    _require_gpu(x, "linear: x")
     if x.dim() == 0 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"{what}: x of shape {tuple(x.shape)} does not fit a weight of {tuple(weight.shape)}")
+        raise ValueError(f"linear: x of shape {tuple(x.shape)} does not fit a weight of {tuple(weight.shape)}")
     if torch.is_autocast_enabled("cuda"):
         dtype = torch.get_autocast_dtype("cuda")
         x, weight = x.to(dtype), weight.to(dtype)
         bias = None if bias is None else bias.to(dtype)
-    _dtype_code(x.dtype, what)
+    _dtype_code(x.dtype, "linear")
     if packed is not None:
-        _require_same_device(packed.values, x.device, f"{what}: packed")
+        _require_same_device(packed.values, x.device, "linear: packed")
         if packed.shape != tuple(x.shape):
-            raise ValueError(f"{what}: packed is of shape {packed.shape}, x of {tuple(x.shape)}")
+            raise ValueError(f"linear: packed is of shape {packed.shape}, x of {tuple(x.shape)}")
     if not (torch.is_grad_enabled()
             and any(t is not None and t.requires_grad for t in (x, weight, bias))):
         return F.linear(x, weight, bias)

@@ -813,43 +813,35 @@ __device__ inline __amdgpu_buffer_rsrc_t buffer(const void* base, int64_t bytes)
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, n, 0x00020000);
 }
 
-__device__ inline void store_out(void* out, int type, int64_t at, float v) {
-  if (type == TFT_F32) static_cast<float*>(out)[at] = v;
-  else if (type == TFT_BF16) static_cast<uint16_t*>(out)[at] = BF16::narrow1(v);
-  else static_cast<uint16_t*>(out)[at] = F16::narrow1(v);
-}
-
 __device__ inline float load_scale(const void* p, int type, int64_t at) {
   if (type == TFT_F32) return static_cast<const float*>(p)[at];
   if (type == TFT_BF16) return BF16::widen1(static_cast<const uint16_t*>(p)[at]);
   return F16::widen1(static_cast<const uint16_t*>(p)[at]);
 }
 
-// Four neighbouring features of one output row, scaled and rounded
-__device__ inline void store_out4(const WgradArgs& a, int64_t o, int64_t f, f32x4 v) {
-  const int n = (int)min((int64_t)a.features - f, (int64_t)4);
-  if (a.column_scale) {
+// Up to four neighbouring features f .. of an output row, scaled and rounded: the slow form, for
+// rows that are no whole number of fours
+__device__ inline void store_out(const WgradArgs& a, int64_t o, int64_t f, const f32x4& v) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) v[i] *= load_scale(a.column_scale, a.scale_type, f + i);
+  for (int i = 0; i < 4; ++i) {
+    if (f + i >= a.features) return;
+    const float x = a.column_scale ? v[i] * load_scale(a.column_scale, a.scale_type, f + i) : v[i];
+    const int64_t at = o * a.features + f + i;
+    if (a.out_type == TFT_F32) static_cast<float*>(a.out)[at] = x;
+    else static_cast<uint16_t*>(a.out)[at] = a.out_type == TFT_BF16 ? BF16::narrow1(x) : F16::narrow1(x);
   }
-  const int64_t at = o * a.features + f;
-  if (n == 4 && a.features % 4 == 0) {
-    if (a.out_type == TFT_F32) {
-      *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = v;
-    } else {
-      uint16_t b[4];
+}
+
+template <typename T>
+__device__ inline void store_four(typename T::elem_t* p, const f32x4& v) {
+  if constexpr (sizeof(typename T::elem_t) == 4) {
+    *reinterpret_cast<f32x4*>(p) = v;
+  } else {
+    uint16_t b[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        b[i] = a.out_type == TFT_BF16 ? BF16::narrow1(v[i]) : F16::narrow1(v[i]);
-      u32x2 w = {b[0] | ((uint32_t)b[1] << 16), b[2] | ((uint32_t)b[3] << 16)};
-      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at) = w;
-    }
-    return;
+    for (int i = 0; i < 4; ++i) b[i] = T::narrow1(v[i]);
+    *reinterpret_cast<u32x2*>(p) = u32x2{b[0] | ((uint32_t)b[1] << 16), b[2] | ((uint32_t)b[3] << 16)};
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < n) store_out(a.out, a.out_type, at + i, v[i]);
 }
 
 // Tile of O output rows x F features, wavefronts in a WO x WF grid.
@@ -884,8 +876,9 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
   if (is_cut) {
     slot = neighbours_on_an_xcd(blockIdx.x - a.whole, a.cut * a.splits);  // split-major
     const uint32_t split = slot / a.cut;
-    step_begin = (uint32_t)((uint64_t)a.steps * split / a.splits);
-    step_end = (uint32_t)((uint64_t)a.steps * (split + 1) / a.splits);
+    const uint32_t each = a.steps / a.splits, more = a.steps - each * a.splits;
+    step_begin = split * each + min(split, more);
+    step_end = step_begin + each + (split < more ? 1 : 0);
     tile_at(a, a.whole + slot - split * a.cut, &tile_o, &tile_f);
   } else {
     tile_at(a, neighbours_on_an_xcd(blockIdx.x, a.whole), &tile_o, &tile_f);
@@ -934,7 +927,7 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
   u32x4 x_reg[kXChunks];
   uint32_t e_reg[kXChunks];
   // D and X are asked for at different times, each as soon as its registers are free
-  auto fetch_d = [&]() {
+  auto fetch_d_into = [&](typename T::raw_t (&d_reg)[kDChunks]) {
     const auto d = buffer(d_at, (left * a.d_stride - o0) * (int64_t)sizeof(elem_t));
 #pragma unroll
     for (int i = 0; i < kDChunks; ++i)
@@ -942,7 +935,7 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
       for (int w = 0; w < (int)sizeof(elem_t) / 2; ++w)
         d_reg[i].w[w] = __builtin_amdgcn_raw_buffer_load_b128(d, d_off[i] + 16 * w, 0, 0);
   };
-  auto fetch_x = [&]() {
+  auto fetch_x_into = [&](u32x4 (&x_reg)[kXChunks], uint32_t (&e_reg)[kXChunks]) {
     const auto x = buffer(x_at, left * a.pitch - f0);
     const auto e = buffer(e_at, left * a.blocks - f0 / kBlock);
 #pragma unroll
@@ -973,6 +966,8 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
     x_at += kTokens * a.pitch;
     e_at += (int64_t)kTokens * a.blocks;
   };
+  auto fetch_d = [&]() { fetch_d_into(d_reg); };
+  auto fetch_x = [&]() { fetch_x_into(x_reg, e_reg); };
   auto stage_d = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < kDChunks; ++i) {
@@ -1047,17 +1042,26 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
   static_assert(kProducts % 2 == 0 && kTokens / 16 % 2 == 0, "the operands' turns close with a step");
   if (step_begin < step_end) {
     int d_now = 0, d_next = 1, d_after = kDirect ? 2 : 0, x_now = 0;
+    // the first two tiles are asked for together: one memory latency before the first product
+    typename T::raw_t d_second[kDChunks];
+    u32x4 x_second[kXChunks];
+    uint32_t e_second[kXChunks];
     if constexpr (kDirect) fetch_d_direct(0);
     else fetch_d();
     fetch_x();
     advance();
-    if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    else stage_d(0);
-    stage_x(0);
     if constexpr (kDirect) fetch_d_direct(1);
-    else fetch_d();
-    fetch_x();
+    else fetch_d_into(d_second);
+    fetch_x_into(x_second, e_second);
     advance();
+    if constexpr (!kDirect) stage_d(0);
+    stage_x(0);
+    if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < kDChunks; ++i)
+      if (!kDirect) d_reg[i] = d_second[i];
+#pragma unroll
+    for (int i = 0; i < kXChunks; ++i) x_reg[i] = x_second[i], e_reg[i] = e_second[i];
     __syncthreads();
     load(0, 0, 0);
     for (uint32_t s = step_begin; s < step_end; ++s) {
@@ -1105,31 +1109,73 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
   float* const turn = reinterpret_cast<float*>(lds) + wave * 32 * kPitch;
   constexpr int kLanes = kWide / 4;  // lanes per row
   const int64_t f = f0 + wave_f + (lane % kLanes) * 4;
-#pragma unroll
-  for (int j = 0; j < kFragO; ++j) {
-#pragma unroll
-    for (int i = 0; i < kFragF; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<f32x4*>(&turn[(lane & 31) * kPitch + i * 32 + q * 8 + (lane >> 5) * 4]) =
-            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+  const int64_t o_lane = wave_o + lane / kLanes;  // this lane's first row; the next one is 64 / kLanes on
+  constexpr int kRows = kLanes / 2;               // of 32 that it stores
+  auto fence = [&]() {  // between lanes of the wavefront, through LDS
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll 4
-    for (int k = 0; k < kLanes / 2; ++k) {
-      const int r = k * (64 / kLanes) + lane / kLanes;
-      const int64_t o = o0 + wave_o + j * 32 + r;
-      const f32x4 v = *reinterpret_cast<const f32x4*>(&turn[r * kPitch + (lane % kLanes) * 4]);
-      if (is_cut)
-        *reinterpret_cast<f32x4*>(a.partial + ((int64_t)slot * O + (wave_o + j * 32 + r)) * F + wave_f +
-                                  (lane % kLanes) * 4) = v;
-      else if (o < a.out_features && f < a.features)
-        store_out4(a, o, f, v);
+  };
+  // store(row of the tile, four features); all rows of a turn are read before the first is stored
+  auto store_all = [&](auto store) {
+#pragma unroll
+    for (int j = 0; j < kFragO; ++j) {
+#pragma unroll
+      for (int i = 0; i < kFragF; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4*>(&turn[(lane & 31) * kPitch + i * 32 + q * 8 + (lane >> 5) * 4]) =
+              f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+      fence();
+      f32x4 v[kRows];
+#pragma unroll
+      for (int k = 0; k < kRows; ++k)
+        v[k] = *reinterpret_cast<const f32x4*>(&turn[(k * (64 / kLanes) + lane / kLanes) * kPitch + (lane % kLanes) * 4]);
+      fence();
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) store(o_lane + j * 32 + k * (64 / kLanes), v[k]);
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  auto store_as = [&](auto type, const f32x4& scale) {
+    typedef decltype(type) Out;
+    typename Out::elem_t* const to = static_cast<typename Out::elem_t*>(a.out) + o0 * a.features + f;
+    const int64_t rows = f < a.features ? (int64_t)a.out_features - o0 : 0;
+    store_all([&](int64_t row, const f32x4& v) {
+      if (row < rows) store_four<Out>(to + row * a.features, v * scale);
+    });
+  };
+  if (is_cut) {
+    float* const to = a.partial + (int64_t)slot * O * F + wave_f + (lane % kLanes) * 4;
+    store_all([&](int64_t row, const f32x4& v) { *reinterpret_cast<f32x4*>(to + row * F) = v; });
+  } else if (a.features % 4 == 0) {
+    f32x4 scale = {1.0f, 1.0f, 1.0f, 1.0f};
+    if (a.column_scale) {
+      const int64_t at = min(f, (int64_t)a.features - 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) scale[i] = load_scale(a.column_scale, a.scale_type, at + i);
+    }
+    if (a.out_type == TFT_BF16) store_as(BF16(), scale);
+    else if (a.out_type == TFT_F16) store_as(F16(), scale);
+    else store_as(F32(), scale);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kFragO; ++j) {
+#pragma unroll
+      for (int i = 0; i < kFragF; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4*>(&turn[(lane & 31) * kPitch + i * 32 + q * 8 + (lane >> 5) * 4]) =
+              f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+      fence();
+#pragma unroll 1
+      for (int k = 0; k < kRows; ++k) {
+        const int r = k * (64 / kLanes) + lane / kLanes;
+        const int64_t o = o0 + wave_o + j * 32 + r;
+        if (o < a.out_features)
+          store_out(a, o, f, *reinterpret_cast<const f32x4*>(&turn[r * kPitch + (lane % kLanes) * 4]));
+      }
+      fence();
+    }
   }
 }
 
@@ -1143,11 +1189,27 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(WgradArgs a) {
   const int64_t o = (int64_t)tile_o * O + in / (F / 4), f = (int64_t)tile_f * F + in % (F / 4) * 4;
   if (o >= a.out_features || f >= a.features) return;
   const float* p = a.partial + ((int64_t)tile * kPerTile + in) * 4;
-  f32x4 v = *reinterpret_cast<const f32x4*>(p);
-#pragma unroll 4
-  for (uint32_t s = 1; s < a.splits; ++s)
-    v += *reinterpret_cast<const f32x4*>(p + (int64_t)s * a.cut * O * F);
-  store_out4(a, o, f, v);
+  const int64_t next = (int64_t)a.cut * O * F;
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t s = 0; s < a.splits; s += 4) {  // four loads in flight
+    f32x4 part[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+      part[i] = s + i < a.splits ? *reinterpret_cast<const f32x4*>(p + (s + i) * next) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) v += part[i];
+  }
+  if (a.features % 4 != 0) {
+    store_out(a, o, f, v);
+    return;
+  }
+  if (a.column_scale)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] *= load_scale(a.column_scale, a.scale_type, f + i);
+  const int64_t to = o * a.features + f;
+  if (a.out_type == TFT_BF16) store_four<BF16>(static_cast<uint16_t*>(a.out) + to, v);
+  else if (a.out_type == TFT_F16) store_four<F16>(static_cast<uint16_t*>(a.out) + to, v);
+  else store_four<F32>(static_cast<float*>(a.out) + to, v);
 }
 
 // ---------------------------------------------------------------------------
@@ -1270,7 +1332,7 @@ constexpr int64_t kCUs = 256;
 // Microseconds that the tiles of one size take with those left over from whole rounds of the chip
 // cut into `splits` pieces along the tokens.  A step of 16 x kProducts tokens takes 0.8 us of a
 // small tile alone on its CU, 1.15 of two beside each other and 1.8 of a large one; a round of
-// workgroups starts and ends in 7; partial tiles are written and read at 7 TB/s and joined by a
+// workgroups starts and ends in 5; partial tiles are written and read at 7 TB/s and joined by a
 // launch of 2.
 double wgrad_time(bool large, int64_t tiles, int64_t steps, int products, int64_t splits) {
   const int64_t at_once = large ? kCUs : 2 * kCUs, size = large ? kLarge : kSmall, pieces = tiles % at_once * splits;
@@ -1279,7 +1341,7 @@ double wgrad_time(bool large, int64_t tiles, int64_t steps, int products, int64_
   if (!pieces) return whole;
   const double each = step * (large ? 1.8 : pieces > kCUs ? 1.15 : 0.8);
   const int64_t rounds = (pieces + at_once - 1) / at_once, longest = (steps + splits - 1) / splits;
-  return whole + rounds * (7.0 + longest * each) + (splits > 1 ? 2.0 + pieces * size * size * 8 / 7e6 : 0.0);
+  return whole + rounds * (5.0 + longest * each) + (splits > 1 ? 2.0 + pieces * size * size * 8 / 7e6 : 0.0);
 }
 
 // Large tiles read LDS less per product and small ones fill the chip with less; which of them, and
