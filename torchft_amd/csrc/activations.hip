@@ -338,6 +338,8 @@ constexpr int kUnpackUnroll = 2;
 constexpr int kPackBlocks = kPackThreads / 16 * kPackUnroll;  // blocks per workgroup
 constexpr int kUnpackBlocks = kPackThreads / 16 * kUnpackUnroll;
 
+// Bound by memory: an element is read once and one byte written.  8192 x 14336 bf16 (353 MB)
+// takes 54 us, 6.5 TB/s; two or one blocks a lane instead of four 55 and 61 us.
 template <typename T, bool S>
 __global__ __launch_bounds__(kPackThreads) void pack_kernel(PackArgs a) {
   const int lane = threadIdx.x & 15;
@@ -378,6 +380,7 @@ struct UnpackArgs {
   Divider per_row;
 };
 
+// Bound by memory like packing: 8192 x 14336 to bf16 takes 56 us, 6.3 TB/s (four blocks a lane 58).
 // W: type of the column scale
 template <typename T, typename W, bool S>
 __global__ __launch_bounds__(kPackThreads) void unpack_kernel(UnpackArgs a) {
@@ -440,8 +443,8 @@ struct NormArgs {
 // 512 features are one wavefront's, four rows to a workgroup and no barrier (Four); longer rows
 // take a workgroup of as many wavefronts as it has 512 features, from 8192 on twice as many
 // features a lane (C = 2).  One chunk of eight features a lane keeps the most wavefronts, and so
-// the most loads, in flight: 16384 x 4096 bf16 with a residual takes 97.7 us with eight
-// wavefronts of one chunk, 101 with four of two, 104 with two of four.
+// the most loads, in flight: 16384 x 4096 bf16 with a residual (604 MB) takes 99 us, 6.1 TB/s, with
+// eight wavefronts of one chunk, 101 with four of two, 104 with two of four.
 template <typename T, bool Four, int C, bool S>
 __global__ __launch_bounds__(Four ? 256 : 1024) void norm_kernel(NormArgs a) {
   const int kTeam = Four ? 64 : blockDim.x;
@@ -544,7 +547,8 @@ struct NormBackArgs {
 // Teams as in norm_kernel.  A workgroup takes rows blockIdx.x, + gridDim.x, ... and keeps the
 // weight gradient of its rows in registers; column_reduce_kernel adds the workgroups' partial
 // sums in a fixed order.  A row is asked for while the one before it is worked on: few rows are
-// in flight, because every workgroup leaves a partial sum of a whole row behind.
+// in flight, because every workgroup leaves a partial sum of a whole row behind.  8192 x 4096 bf16
+// with grad_h (235 MB) takes 39 us, 6.0 TB/s, and 4.7 for the partial sums; without asking ahead 69.
 template <typename T, bool Four, int C>
 __global__ __launch_bounds__(Four ? 256 : 1024) void norm_back_kernel(NormBackArgs a) {
   constexpr int kRows = Four ? 4 : 1;
@@ -852,7 +856,18 @@ __device__ inline void store_four(typename T::elem_t* p, const f32x4& v) {
 // operands: lanes 0 .. 31 hold a product's first eight tokens of 32 columns, lanes 32 .. 63 the
 // other eight.  Rows of a tile are units of 16 columns (32 bytes); unit u of token t lies at
 // u ^ spread(t), so that the four rows of a transposing read, and the two units that lanes 0 .. 31
-// read together, lie on different banks.
+// read together, lie on different banks (248 of LDS's 256 bytes a cycle; 64 with every unit u at u).
+//
+// What bounds it.  A step of a large tile is 2048 cycles of matrix instructions on every SIMD.
+// Next to them LDS gives out 192 KiB and takes in 64 (about 770 and 830 cycles), and the vector
+// memory path brings 48 KiB (about 770), all from the same two wavefronts per SIMD.  8192 tokens,
+// 14336 x 4096 bf16 take 775 to 830 us from box to box (1160 to 1240 TFLOP/s): the matrix
+// units are busy about 55 % of the time at the 2.0 GHz that the power limit leaves (zeros in place
+// of the data: 2.4 GHz, 630 us).  On the same box torch's product of these operands as they lie,
+// already unpacked, takes 997 us, and with both operands turned beforehand 650 to 710.
+// Tried and no faster: two groups of wavefronts that take turns at the matrix units (807 to
+// 860 us), four wavefronts of 128 x 128 with every instruction's place laid down by hand (875),
+// D through registers (850), half the loads of exponents (822).
 __device__ inline int spread(int t) { return (t & 3) | ((t & 1) << 2); }
 
 template <typename T, int O, int F, int WO, int WF>
@@ -945,7 +960,8 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
     }
   };
   // D past the registers, into buffer `to`.  The compiler does not know of these loads: who reads
-  // the buffer has waited for them by hand.
+  // the buffer has waited for them by hand.  (With the compiler's own form of this load every
+  // barrier waits for all of them.)  Nothing else here uses M0, which gfx950's LDS accesses ignore.
   auto fetch_d_direct = [&](int to) {
     const uint64_t base = (uint64_t)d_at;
     const int64_t bytes = (left * a.d_stride - o0) * (int64_t)sizeof(elem_t);
@@ -1179,7 +1195,8 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
   }
 }
 
-// Joins the partial products of the cut tiles, in the order of the sum.
+// Joins the partial products of the cut tiles, in the order of the sum.  Bound by memory: 128 large
+// tiles in two pieces (67 MB in, 17 out) take 18 us.
 template <int O, int F>
 __global__ __launch_bounds__(256) void wgrad_join_kernel(WgradArgs a) {
   constexpr uint32_t kPerTile = O * F / 4;
@@ -1346,9 +1363,9 @@ double wgrad_time(bool large, int64_t tiles, int64_t steps, int products, int64_
 
 // Large tiles read LDS less per product and small ones fill the chip with less; which of them, and
 // how many pieces, is the least of the times above.  Measured, us, large tiles in their best number
-// of pieces / small ones: 8192 tokens, 4096 x 4096 bf16 242 (1) / 313 (1); 8192, 1024 x 4096
-// 82 (4) / 90 (2); 4096, 2048 x 2048 fp16 78 (4) / 91 (2); 1024, 768 x 768 bf16 21 (5) / 15 (3);
-// 1000, 1001 x 768 fp32 31 (10) / 28 (3).
+// of pieces / small ones in theirs: 8192 tokens, 4096 x 4096 bf16 225 (1) / 306 (2); 8192,
+// 1024 x 4096 80 (4) / 88 (2); 4096, 2048 x 2048 fp16 80 (4) / 90 (2); 1024, 768 x 768 bf16
+// 21 (5) / 15 (3); 1000, 1001 x 768 fp32 31 (10) / 28 (3).
 WgradPlan plan_wgrad(int64_t rows, int64_t out_features, int64_t features, int64_t grad_stride,
                      int dtype, bool aligned) {
   WgradPlan p{};
