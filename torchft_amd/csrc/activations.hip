@@ -794,6 +794,7 @@ struct WgradArgs {
   uint32_t whole, cut, splits;  // tiles of one workgroup each, tiles of `splits` workgroups each
   uint32_t steps;
   int scale_type, out_type;  // TFT_F32 ...
+  int partial_past_caches;
 };
 
 // Workgroup ids go round the 8 XCDs in turn; this gives each of them a run of neighbouring
@@ -1162,7 +1163,12 @@ __global__ __launch_bounds__(64 * WO * WF, 1) void wgrad_kernel(WgradArgs a) {
   };
   if (is_cut) {
     float* const to = a.partial + (int64_t)slot * O * F + wave_f + (lane % kLanes) * 4;
-    store_all([&](int64_t row, const f32x4& v) { *reinterpret_cast<f32x4*>(to + row * F) = v; });
+    if (a.partial_past_caches)
+      store_all([&](int64_t row, const f32x4& v) {
+        __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(to + row * F));
+      });
+    else
+      store_all([&](int64_t row, const f32x4& v) { *reinterpret_cast<f32x4*>(to + row * F) = v; });
   } else if (a.features % 4 == 0) {
     f32x4 scale = {1.0f, 1.0f, 1.0f, 1.0f};
     if (a.column_scale) {
@@ -1333,6 +1339,12 @@ uint32_t column_sum_groups(int64_t rows, int64_t columns) {
   if (g > (rows + 7) / 8) g = (rows + 7) / 8;
   return (uint32_t)(g < 1 ? 1 : g);
 }
+
+// Partial tiles that fit the XCDs' L2 together are written past it: the kernel's end would wait for
+// their write-back (1000 tokens, 1001 x 768 fp32, 16 MB: 27 us so, 30 through L2; 1024, 768 x 768
+// bf16, 7 MB: 15.3 and 16.3).  More of them are written back while the kernel runs, and the join
+// finds the rest in the cache (8192, 1024 x 4096, 67 MB: 80.6 and 77.2).
+constexpr int64_t kL2Bytes = 32ll << 20;
 
 // How a weight gradient is cut.
 struct WgradPlan {
@@ -1641,7 +1653,8 @@ int tft_linear_weight_grad(void* grad_weight, void* workspace, int64_t workspace
                     static_cast<const uint8_t*>(exponents), column_scale, grad_weight,
                     reinterpret_cast<float*>(static_cast<char*>(workspace) + p.aligned_bytes), rows, p.padded, pitch,
                     (uint32_t)out_features, (uint32_t)features, (uint32_t)((features + kBlock - 1) / kBlock),
-                    p.tiles_o, p.tiles_f, p.whole, p.cut, p.splits, p.steps, scale_dtype, out_dtype};
+                    p.tiles_o, p.tiles_f, p.whole, p.cut, p.splits, p.steps, scale_dtype, out_dtype,
+                    p.partial_bytes <= kL2Bytes ? 1 : 0};
   if (dtype == TFT_F32) return launch_wgrad<F32>(what, a, p, align, s);
   if (dtype == TFT_BF16) return launch_wgrad<BF16>(what, a, p, align, s);
   return launch_wgrad<F16>(what, a, p, align, s);
