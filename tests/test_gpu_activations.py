@@ -432,6 +432,20 @@ def _tail_packed(p, features):
     return PackedActivation(p.values[:, :features].contiguous(), p.exponents[:, :1].contiguous(), features)
 
 
+def test_output_past_32_bits(device):
+    """2.4e9 elements of a weight gradient: its last rows against the checker."""
+    rows, out_features, features = 20, 590_000, 4096
+    d = torch.zeros(rows, out_features, dtype=torch.bfloat16, device=device)
+    d[:, -70:] = randn(1, rows, 70, dtype=torch.bfloat16).to(device)
+    p = A.pack(randn(2, rows, features).to(device))
+    got = A.linear_weight_grad(d, p)
+    n = p.unpack().cpu()
+    want = O.linear_weight_grad(d[:, -70:].cpu(), n)
+    tol = O.linear_weight_grad(d[:, -70:].cpu().abs(), n.abs()) * 200 * ULP32
+    assert_within(got[-70:], want, tol + rounding(want, torch.bfloat16) * (1 + 2.0 ** -10), "last rows")
+    assert not bool(got[:-70].any())
+
+
 def test_norm_offsets_past_32_bits(device):
     rows, features = (1 << 20) + 3, 4160
     x = torch.ones(rows, features, dtype=torch.bfloat16, device=device)
@@ -592,6 +606,57 @@ def test_packed_norm_output_is_shared_by_the_layers_behind_it(device):
         y.mul_(2.0)  # written to since: the layer packs what it sees
     gw, = torch.autograd.grad((a(y) * ga).sum(), (a.weight,))
     assert_bits_equal(gw, A.linear_weight_grad(ga, A.pack(y.detach())))
+
+
+def test_modules_without_gradients_and_without_rows(device):
+    model = A.pack_activations(small_block(torch.float32, device))
+    x = randn(1, 5, 192).to(device)
+    want = model(x).detach()
+    with torch.inference_mode():
+        assert torch.equal(model(x), want)
+    with torch.no_grad():
+        assert torch.equal(model(x), want)
+    empty = torch.zeros(0, 192, device=device, requires_grad=True)
+    grads = torch.autograd.grad(model(empty).sum(), [empty, *model.parameters()])
+    assert grads[0].shape == (0, 192) and not any(bool(g.any()) for g in grads)
+    norm = A.pack_activations(nn.RMSNorm(192, elementwise_affine=False).to(device))
+    row = x[0].clone().requires_grad_()  # one row, no weight
+    y = norm(row)
+    assert y.shape == (192,) and torch.autograd.grad(y.sum(), row)[0].shape == (192,)
+
+
+def test_two_threads_at_once(device):
+    """Calls keep nothing between them: two threads on two streams get what one gets."""
+    import threading
+
+    data = [(randn(k, 400, 640).to(device), randn(k + 9, 400, 136, dtype=torch.float16).to(device)) for k in (1, 2)]
+
+    def work(x, d):
+        y, _, p, rstd = A.rms_norm_forward(x, None, 1e-5)
+        return y, A.rms_norm_backward(x, p, rstd)[0], A.linear_weight_grad(d, p), p.unpack()
+
+    want = [work(*d) for d in data]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def run(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[k] = work(*data[k])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # shown by the assertion below
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for g, w in zip(got, want):
+        for a, b in zip(g, w):
+            assert_bits_equal(a, b)
 
 
 def test_writing_to_a_norms_weight_before_the_backward_pass_is_an_error(device):

@@ -545,8 +545,10 @@ class Linear(nn.Linear):
     """``torch.nn.Linear`` that keeps its input in 8 bits for the weight gradient."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        packed, version = getattr(x, _CARRIED, (None, None))
-        return linear(x, self.weight, self.bias, packed if version == x._version else None)
+        carried = getattr(x, _CARRIED, None)
+        if carried is not None and carried[1] == x._version:
+            return linear(x, self.weight, self.bias, carried[0])
+        return linear(x, self.weight, self.bias)
 
 
 def pack_activations(module: nn.Module) -> nn.Module:
