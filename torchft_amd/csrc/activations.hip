@@ -1394,7 +1394,7 @@ WgradPlan plan_wgrad(int64_t rows, int64_t out_features, int64_t features, int64
     const int64_t across = (out_features + size - 1) / size, along = (features + size - 1) / size;
     const int64_t tiles = across * along, over = tiles % at_once;
     const int64_t most = over == 0 ? 1 : at_once / over < p.steps ? at_once / over : p.steps > 1 ? p.steps : 1;
-    for (int64_t splits = 1; splits <= most; ++splits) {
+    for (int64_t splits = 1; splits <= most; splits += 1 + splits / 8) {
       const double time = wgrad_time(large, tiles, p.steps, tokens / 16 * parts, splits);
       if (best != 0.0 && time >= best) continue;
       best = time;
