@@ -213,6 +213,22 @@ def test_norm_forms(device, dtype, weight_dtype, rows, features, with_residual):
     check_norm(device, rows, features, dtype, weight_dtype, with_residual, 3, 1, seed=rows)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [1.0, 0.02, 0.001])
+def test_norm_without_eps_is_torchs(device, dtype, size):
+    """Rows so small that eps decides their norm (at 0.001 it is 12 % of the mean square): the
+    module before and after its conversion, both against the definition with fp32's epsilon."""
+    x = randn(1, 5, 4096, dtype=dtype, scale=size)
+    norm = nn.RMSNorm(4096).to(device, dtype)
+    before = norm(x.to(device)).detach()
+    after = A.pack_activations(norm)(x.to(device)).detach()
+    want = O.rms_norm(x, None, torch.finfo(torch.float32).eps)[0]
+    tol = want.abs() * (45 / 2 + 5) * 2.0 ** -24 + rounding(want, dtype) * (1 + 2.0 ** -10)
+    assert_within(before, want, tol, "torch's norm")
+    assert_within(after, want, tol, "the converted norm")
+    assert_bits_equal(A.rms_norm_forward(x.to(device))[0], after)
+
+
 def test_norm_of_rows_of_zeros_and_nan(device):
     x = randn(1, 4, 200)
     x[1] = 0.0

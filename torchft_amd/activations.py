@@ -264,8 +264,9 @@ def rms_norm_forward(
 ) -> Tuple[torch.Tensor, torch.Tensor, Optional[PackedActivation], torch.Tensor]:
     """(y, h, packed, rstd) with h = x + residual rounded to x's type (x itself without a
     residual), rstd = 1 / sqrt(mean(h^2) + eps) in fp32 of [rows], y = h * rstd * weight, and the
-    normalised rows h * rstd packed with ``weight`` as their column scale.  ``eps=None`` is the
-    type's machine epsilon, as in ``torch.nn.RMSNorm``.  No autograd: see :func:`rms_norm`."""
+    normalised rows h * rstd packed with ``weight`` as their column scale.  ``eps=None`` is fp32's
+    machine epsilon whatever x's type, as torch's norm takes that of the type it computes in.  No
+    autograd: see :func:`rms_norm`."""
     rows, features, stride = _matrix(x, "rms_norm: x")
     dtype, device = x.dtype, x.device
     code = _dtype_code(dtype, "rms_norm")
@@ -274,7 +275,7 @@ def rms_norm_forward(
     _vector(weight, features, device, "rms_norm: weight")
     _check_norm_weight(weight, dtype, "rms_norm")
     if eps is None:
-        eps = torch.finfo(dtype).eps
+        eps = torch.finfo(torch.float32).eps
     if not eps >= 0.0:
         raise ValueError(f"rms_norm: eps must be at least 0, got {eps}")
     residual_stride = 0
