@@ -372,6 +372,19 @@ def test_weight_gradient_of_large_layers(device, rows, out_features, features, d
     big_wgrad(device, rows, out_features, features, dtype)
 
 
+@pytest.mark.parametrize("dtype,stride", [(torch.bfloat16, 1 << 24), (torch.float16, 1 << 24), (torch.float32, 1 << 23),
+                                          (torch.bfloat16, (1 << 24) - 8), (torch.float32, (1 << 23) + 1)])
+def test_weight_gradient_of_rows_far_apart(device, dtype, stride):
+    """A step's slice of a gradient that holds many steps: 32 MB and more from row to row."""
+    d = randn(2, 70, 64, dtype=dtype).to(device)
+    p = A.pack(randn(1, 70, 200).to(device))
+    far = torch.empty(69 * stride + 64, dtype=dtype, device=device).as_strided((70, 64), (stride, 1))
+    far.copy_(d)
+    assert_bits_equal(A.linear_weight_grad(far, p), A.linear_weight_grad(d, p))
+    steps = far.unsqueeze(1)  # [70, 1, 64]: the rows are a view's
+    assert_bits_equal(A.linear_weight_grad(steps, p), A.linear_weight_grad(d, p))
+
+
 def test_weight_gradient_of_expanded_and_empty(device):
     p = A.pack(randn(1, 90, 200).to(device))
     row = randn(2, 1, 64, dtype=torch.bfloat16).to(device)

@@ -32,6 +32,7 @@ from . import _native
 
 BLOCK = 128  # features that share a scale
 MAX_NORM_FEATURES = 16384
+_WGRAD_ROW_BYTES = 1 << 25  # the weight gradient's kernel addresses 64 rows of a gradient with 31 bits
 
 _DTYPES = {
     torch.float32: _native.TFT_F32,
@@ -363,6 +364,8 @@ def linear_weight_grad(
     dtype = grad_out.dtype if dtype is None else dtype
     out_code = _dtype_code(dtype, "linear_weight_grad")
     device = grad_out.device
+    if stride > out_features and stride * grad_out.element_size() >= _WGRAD_ROW_BYTES:
+        grad_out, stride = grad_out.contiguous(), out_features
     if rows != packed.rows:
         raise ValueError(f"linear_weight_grad: grad_out has {rows} rows, packed {packed.rows}")
     _require_same_device(packed.values, device, "linear_weight_grad: packed")
