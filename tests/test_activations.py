@@ -261,6 +261,16 @@ def test_c_entries_refuse_without_a_gpu():
     assert space(at, 4096, 128, 128, 128, 128, 1) >= 2 * 128 * 128 * 4
 
 
+def test_weight_gradients_of_more_tiles_than_a_launch_holds_are_refused():
+    """2^27 tiles of 512 threads: over the 2^32 threads of a dispatch (16 TB of gradient)."""
+    lib = _native.lib()
+    buf = ctypes.create_string_buffer(4096)
+    at = (ctypes.addressof(buf) + 255) // 256 * 256
+    rc = lib.tft_linear_weight_grad(at, at, 1 << 62, at, at, at, None, 1, 1 << 23, 1 << 20, 1 << 23, 1 << 20,
+                                    1, 0, 1, None)
+    assert rc == -2 and b"tiles" in lib.tft_last_error()
+
+
 # --- modules ------------------------------------------------------------------------------------
 
 

@@ -488,6 +488,62 @@ def test_norm_offsets_past_32_bits(device):
     assert torch.equal(gx[-3:], sgx)
 
 
+def test_norm_of_more_rows_than_a_launch_holds(device):
+    """2^26 rows of a wavefront each are 2^32 threads, one more than a dispatch can have."""
+    rows, features, tail = (1 << 26) + 5, 8, 70
+    g = torch.Generator(device=device).manual_seed(1)
+    x = torch.randn(rows, features, generator=g, device=device, dtype=torch.bfloat16)
+    r = torch.randn(rows, features, generator=g, device=device, dtype=torch.bfloat16)
+    w = (1 + 0.3 * randn(2, features)).to(device)
+    y, h, p, rstd = A.rms_norm_forward(x, w, 1e-5, r)
+    for part in (slice(rows - tail, rows), slice((1 << 26) - 40, (1 << 26) - 4), slice(0, tail)):
+        sy, sh, sp, srstd = A.rms_norm_forward(x[part].contiguous(), w, 1e-5, r[part].contiguous())
+        assert_bits_equal(y[part], sy)
+        assert_bits_equal(h[part], sh)
+        assert_bits_equal(rstd[part], srstd)
+        assert_bits_equal(p.values[part].view(torch.uint8), sp.values.view(torch.uint8))
+        assert_bits_equal(p.exponents[part], sp.exponents)
+    gx, gw = A.rms_norm_backward(x, p, rstd, r)
+    sgx, _ = A.rms_norm_backward(x[-tail:].contiguous(), A.rms_norm_forward(x[-tail:], w, 1e-5, r[-tail:])[2],
+                                 rstd[-tail:].contiguous(), r[-tail:])
+    assert_bits_equal(gx[-tail:], sgx)
+
+
+def test_norm_of_more_wide_rows_than_a_launch_holds(device):
+    """2^25 rows of two wavefronts each; the rows of x overlap, each starts one element on."""
+    rows, features, tail = (1 << 25) + 3, 520, 70
+    g = torch.Generator(device=device).manual_seed(1)
+    x = torch.randn(rows + features, generator=g, device=device, dtype=torch.bfloat16).as_strided((rows, features), (1, 1))
+    y, _, _, rstd = A.rms_norm_forward(x, None, 1e-5, pack=False)
+    for part in (slice(rows - tail, rows), slice((1 << 25) - 40, (1 << 25)), slice(0, tail)):
+        sy, _, _, srstd = A.rms_norm_forward(x[part].contiguous(), None, 1e-5, pack=False)
+        assert_bits_equal(y[part], sy)
+        assert_bits_equal(rstd[part], srstd)
+    del x, y
+    torch.cuda.empty_cache()
+
+
+def test_packing_of_more_blocks_than_a_launch_holds(device):
+    """2^30 blocks of sixteen lanes; unpacking reaches the same at half as many.  One small whole
+    number a block: it is kept exactly."""
+    rows = (1 << 30) + 70
+    x = torch.randint(1, 8, (rows, 1), device=device, dtype=torch.int8).bfloat16()
+    p = A.pack(x)
+    back = p.unpack()
+    assert torch.equal(back, x)
+    small = A.pack(x[-50:])
+    assert torch.equal(p.values[-50:].view(torch.uint8), small.values.view(torch.uint8))
+    del x, p, back
+    torch.cuda.empty_cache()
+
+
+def test_column_sum_of_more_columns_than_a_launch_holds(device):
+    columns = (1 << 27) + 40
+    x = torch.randint(-7, 8, (10, columns), device=device, dtype=torch.int8).bfloat16()
+    assert torch.equal(A.column_sum(x, torch.float32), x.float().sum(dim=0))
+    torch.cuda.empty_cache()
+
+
 def test_calls_run_on_the_current_stream_and_repeat(device):
     x, d = randn(1, 300, 1000).to(device), randn(2, 300, 257).to(device)
     w = torch.ones(1000, device=device)

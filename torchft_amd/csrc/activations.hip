@@ -666,17 +666,17 @@ __global__ __launch_bounds__(Four ? 256 : 1024) void norm_back_kernel(NormBackAr
 }
 
 // out[c] = sum over g of partial[g][c], g in fixed order: 32 columns and 32 row lanes per
-// workgroup, the row lanes joined through LDS.
+// workgroup, the row lanes joined through LDS.  `pitch` floats from one g to the next.
 template <typename T>
-__global__ __launch_bounds__(1024) void column_reduce_kernel(const float* partial, void* out,
-                                                             uint32_t groups, int64_t columns) {
+__global__ __launch_bounds__(1024) void column_reduce_kernel(const float* partial, void* out, uint32_t groups,
+                                                             int64_t columns, int64_t pitch) {
   __shared__ float part[32][33];
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int64_t col = (int64_t)blockIdx.x * 32 + x;
   float s = 0.0f;
   if (col < columns)
 #pragma unroll 8
-    for (uint32_t g = y; g < groups; g += 32) s += partial[(int64_t)g * columns + col];
+    for (uint32_t g = y; g < groups; g += 32) s += partial[(int64_t)g * pitch + col];
   part[y][x] = s;
   __syncthreads();
   if (y || col >= columns) return;
@@ -1287,20 +1287,51 @@ int launch(const char* what, const void* kernel, dim3 grid, int threads, void** 
   return TFT_OK;
 }
 
+// A dispatch counts its threads with 32 bits.  Calls of more rows than fit into one are launched in
+// slices: rows are independent of each other, so a slice is the same call of fewer rows.
+int64_t most_groups(int threads) { return 0xffffffffll / threads; }
+
+// launch_slice(first row, rows) for slices of at most `most` rows
+template <typename F>
+int in_slices(int64_t rows, int64_t most, F launch_slice) {
+  for (int64_t first = 0; first < rows; first += most)
+    if (int rc = launch_slice(first, rows - first < most ? rows - first : most)) return rc;
+  return TFT_OK;
+}
+
+const void* row_at(const void* p, int64_t row, int64_t stride, int dtype) {
+  return p ? static_cast<const char*>(p) + row * stride * esize(dtype) : nullptr;
+}
+
+void* row_at(void* p, int64_t row, int64_t stride, int dtype) {
+  return p ? static_cast<char*>(p) + row * stride * esize(dtype) : nullptr;
+}
+
 #define TFT_KERNEL(...) reinterpret_cast<const void*>(&__VA_ARGS__)
 
 // Threads of a workgroup for rows of so many features, `chunks` of eight a lane
 int norm_threads(int features, int chunks) { return (features + 512 * chunks - 1) / (512 * chunks) * 64; }
 
 template <typename T, bool S>
-int launch_norm(const char* what, const NormArgs& a, hipStream_t s) {
-  NormArgs args = a;
-  void* params[] = {&args};
-  if (a.features <= 512)
-    return launch(what, TFT_KERNEL(norm_kernel<T, true, 1, S>), dim3((a.rows + 3) / 4), 256, params, s);
-  if (a.features <= 8192)
-    return launch(what, TFT_KERNEL(norm_kernel<T, false, 1, S>), dim3(a.rows), norm_threads(a.features, 1), params, s);
-  return launch(what, TFT_KERNEL(norm_kernel<T, false, 2, S>), dim3(a.rows), norm_threads(a.features, 2), params, s);
+int launch_norm(const char* what, const NormArgs& a, int dtype, hipStream_t s) {
+  const bool four = a.features <= 512;  // rows to a workgroup
+  const int chunks = a.features <= 8192 ? 1 : 2, threads = four ? 256 : norm_threads(a.features, chunks);
+  const int64_t blocks = (a.features + kBlock - 1) / kBlock;
+  return in_slices(a.rows, most_groups(threads) * (four ? 4 : 1), [&](int64_t first, int64_t rows) {
+    NormArgs args = a;
+    args.rows = (uint32_t)rows;
+    args.x = row_at(a.x, first, a.x_stride, dtype);
+    args.residual = row_at(a.residual, first, a.residual_stride, dtype);
+    args.y = row_at(a.y, first, a.features, dtype);
+    args.h = row_at(a.h, first, a.features, dtype);
+    args.values = a.values ? a.values + first * a.pitch : nullptr;
+    args.exponents = a.exponents ? a.exponents + first * blocks : nullptr;
+    args.rstd = a.rstd ? a.rstd + first : nullptr;
+    void* params[] = {&args};
+    if (four) return launch(what, TFT_KERNEL(norm_kernel<T, true, 1, S>), dim3((args.rows + 3) / 4), threads, params, s);
+    return launch(what, chunks == 1 ? TFT_KERNEL(norm_kernel<T, false, 1, S>) : TFT_KERNEL(norm_kernel<T, false, 2, S>),
+                  dim3(args.rows), threads, params, s);
+  });
 }
 
 // Two workgroups a CU: more of them hide more of a row's latency and leave more partial sums
@@ -1325,12 +1356,16 @@ int launch_norm_back(const char* what, const NormBackArgs& a, hipStream_t s) {
 
 int launch_column_reduce(const char* what, const float* partial, void* out, uint32_t groups,
                          int64_t columns, int dtype, hipStream_t s) {
-  void* params[] = {&partial, &out, &groups, &columns};
-  const dim3 grid((uint32_t)((columns + 31) / 32));
   const void* k = dtype == TFT_F32 ? TFT_KERNEL(column_reduce_kernel<F32>)
                   : dtype == TFT_BF16 ? TFT_KERNEL(column_reduce_kernel<BF16>)
                                       : TFT_KERNEL(column_reduce_kernel<F16>);
-  return launch(what, k, grid, 1024, params, s);
+  return in_slices(columns, most_groups(1024) * 32, [&](int64_t first, int64_t n) {  // of columns
+    const float* from = groups ? partial + first : nullptr;
+    void* to = row_at(out, first, 1, dtype);
+    int64_t pitch = columns;
+    void* params[] = {&from, &to, &groups, &n, &pitch};
+    return launch(what, k, dim3((uint32_t)((n + 31) / 32)), 1024, params, s);
+  });
 }
 
 uint32_t column_sum_groups(int64_t rows, int64_t columns) {
@@ -1447,15 +1482,19 @@ int tft_pack_e4m3(void* values, void* exponents, const void* x, int64_t rows, in
   if (!x || misaligned(x, dtype)) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: x is NULL or misaligned", what);
   if (x_row_stride < 0) return fail(TFT_ERR_INVALID_ARGUMENT, "%s: negative row stride", what);
   const uint32_t per_row = (uint32_t)((features + kBlock - 1) / kBlock);
-  PackArgs a{x, static_cast<uint8_t*>(values), static_cast<uint8_t*>(exponents), features, x_row_stride,
-             pitch, (uint32_t)(rows * per_row), make_divider(per_row)};
-  void* params[] = {&a};
-  const dim3 grid((a.blocks + kPackBlocks - 1) / kPackBlocks);
   const bool far = rows * features * (esize(dtype) + 1) >= kLastLevelCache;
 #define TFT_PACK(T) (far ? TFT_KERNEL(pack_kernel<T, true>) : TFT_KERNEL(pack_kernel<T, false>))
   const void* k = dtype == TFT_F32 ? TFT_PACK(F32) : dtype == TFT_BF16 ? TFT_PACK(BF16) : TFT_PACK(F16);
 #undef TFT_PACK
-  return launch(what, k, grid, kPackThreads, params, static_cast<hipStream_t>(stream));
+  // a row has at most 2^24 blocks, far less than one launch
+  return in_slices(rows, most_groups(kPackThreads) * kPackBlocks / per_row, [&](int64_t first, int64_t n) {
+    PackArgs a{row_at(x, first, x_row_stride, dtype), static_cast<uint8_t*>(values) + first * pitch,
+               static_cast<uint8_t*>(exponents) + first * per_row, features, x_row_stride, pitch,
+               (uint32_t)(n * per_row), make_divider(per_row)};
+    void* params[] = {&a};
+    return launch(what, k, dim3((a.blocks + kPackBlocks - 1) / kPackBlocks), kPackThreads, params,
+                  static_cast<hipStream_t>(stream));
+  });
 }
 
 int tft_unpack_e4m3(void* out, const void* values, const void* exponents, const void* column_scale,
@@ -1470,10 +1509,6 @@ int tft_unpack_e4m3(void* out, const void* values, const void* exponents, const 
   if (column_scale && misaligned(column_scale, scale_dtype))
     return fail(TFT_ERR_INVALID_ARGUMENT, "%s: column_scale is misaligned", what);
   const uint32_t per_row = (uint32_t)((features + kBlock - 1) / kBlock);
-  UnpackArgs a{out, static_cast<const uint8_t*>(values), static_cast<const uint8_t*>(exponents), column_scale,
-               features, pitch, (uint32_t)(rows * per_row), make_divider(per_row)};
-  void* params[] = {&a};
-  const dim3 grid((a.blocks + kUnpackBlocks - 1) / kUnpackBlocks);
   const int st = column_scale ? scale_dtype : TFT_F32;
   const bool far = rows * features * (esize(dtype) + 1) >= kLastLevelCache;
 #define TFT_UNPACK2(T, W) (far ? TFT_KERNEL(unpack_kernel<T, W, true>) : TFT_KERNEL(unpack_kernel<T, W, false>))
@@ -1484,7 +1519,14 @@ int tft_unpack_e4m3(void* out, const void* values, const void* exponents, const 
   const void* k = dtype == TFT_F32 ? TFT_UNPACK(F32) : dtype == TFT_BF16 ? TFT_UNPACK(BF16) : TFT_UNPACK(F16);
 #undef TFT_UNPACK
 #undef TFT_UNPACK2
-  return launch(what, k, grid, kPackThreads, params, static_cast<hipStream_t>(stream));
+  return in_slices(rows, most_groups(kPackThreads) * kUnpackBlocks / per_row, [&](int64_t first, int64_t n) {
+    UnpackArgs a{row_at(out, first, features, dtype), static_cast<const uint8_t*>(values) + first * pitch,
+                 static_cast<const uint8_t*>(exponents) + first * per_row, column_scale, features, pitch,
+                 (uint32_t)(n * per_row), make_divider(per_row)};
+    void* params[] = {&a};
+    return launch(what, k, dim3((a.blocks + kUnpackBlocks - 1) / kUnpackBlocks), kPackThreads, params,
+                  static_cast<hipStream_t>(stream));
+  });
 }
 
 int tft_rms_norm(void* y, void* h, void* values, void* exponents, float* rstd, const void* x,
@@ -1518,7 +1560,7 @@ int tft_rms_norm(void* y, void* h, void* values, void* exponents, float* rstd, c
              weight_dtype == TFT_F32 ? 1 : 0, eps};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool far = rows * features * (esize(dtype) * (residual ? 4 : 2) + (values ? 1 : 0)) >= kLastLevelCache;
-#define TFT_NORM(T) (far ? launch_norm<T, true>(what, a, s) : launch_norm<T, false>(what, a, s))
+#define TFT_NORM(T) (far ? launch_norm<T, true>(what, a, dtype, s) : launch_norm<T, false>(what, a, dtype, s))
   return dtype == TFT_F32 ? TFT_NORM(F32) : dtype == TFT_BF16 ? TFT_NORM(BF16) : TFT_NORM(F16);
 #undef TFT_NORM
 }
@@ -1640,7 +1682,8 @@ int tft_linear_weight_grad(void* grad_weight, void* workspace, int64_t workspace
   if (p.padded * esize(dtype) * 64 >= (1ll << 31) || pitch * 64 >= (1ll << 31))
     return fail(TFT_ERR_UNSUPPORTED, "%s: rows of %lld gradients or %lld packed values are too long", what,
                 (long long)p.padded, (long long)pitch);
-  if ((int64_t)p.tiles_o * p.tiles_f * 4 >= (1ll << 31))
+  if ((int64_t)p.tiles_o * p.tiles_f * 4 >= (1ll << 31) ||
+      p.whole + (int64_t)p.cut * p.splits > most_groups(p.large ? 512 : 256))
     return fail(TFT_ERR_UNSUPPORTED, "%s: too many tiles for one grid", what);
   const int64_t needed = p.aligned_bytes + p.partial_bytes;
   if (needed && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < needed))
