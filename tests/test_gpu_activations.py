@@ -753,6 +753,23 @@ def test_writing_to_a_norms_weight_before_the_backward_pass_is_an_error(device):
         out.sum().backward()
 
 
+def test_writing_to_a_norms_weight_before_the_layer_behind_it(device):
+    """The packed rows are to be multiplied with the weight that the norm's output was made with."""
+    norm, lin = A.RMSNorm(130).to(device), A.Linear(130, 8).to(device)
+    g = randn(2, 6, 8).to(device)
+    y = norm(randn(1, 6, 130).to(device))
+    with torch.no_grad():
+        norm.weight.mul_(3.0)
+    gw, = torch.autograd.grad((lin(y) * g).sum(), (lin.weight,))
+    assert_bits_equal(gw, A.linear_weight_grad(g, A.pack(y.detach())))
+    out = A.rms_norm(randn(1, 6, 130).to(device), norm.weight)
+    A.linear(out.y, lin.weight, packed=out.packed)
+    with torch.no_grad():
+        norm.weight.mul_(2.0)
+    with pytest.raises(ValueError, match="written to since"):
+        A.linear(out.y, lin.weight, packed=out.packed)
+
+
 def test_autocast(device):
     lin = A.Linear(130, 16).to(device)
     x = randn(1, 9, 130).to(device)

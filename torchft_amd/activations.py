@@ -143,13 +143,18 @@ def _vector(t: Optional[torch.Tensor], features: int, device: torch.device, what
     _dtype_code(t.dtype, what)
 
 
+def _version(t: Optional[torch.Tensor]) -> Optional[int]:
+    """How often t was written to, as far as torch counts (not for tensors of inference mode)."""
+    return None if t is None or t.is_inference() else t._version
+
+
 class PackedActivation:
     """An activation in 8 bits: E4M3 ``values`` of [rows, features rounded up to 16] and biased
     ``exponents`` (uint8) of [rows, blocks of 128 features].  An element stands for
     ``value * 2 ** (exponent - 127)``, times ``column_scale`` of its feature where there is one
     (a norm's weight).  ``shape`` is the packed tensor's and ``dtype`` its type."""
 
-    __slots__ = ("values", "exponents", "features", "shape", "dtype", "column_scale")
+    __slots__ = ("values", "exponents", "features", "shape", "dtype", "column_scale", "_scale_version")
 
     def __init__(
         self,
@@ -193,6 +198,7 @@ class PackedActivation:
         self.shape = shape
         self.dtype = dtype
         self.column_scale = column_scale
+        self._scale_version = _version(column_scale)
 
     @property
     def rows(self) -> int:
@@ -205,6 +211,11 @@ class PackedActivation:
     @property
     def nbytes(self) -> int:
         return self.values.numel() + self.exponents.numel()
+
+    def _scale_is_as_packed(self) -> bool:
+        """Whether the column scale (a norm's live weight) is still the one that the packed
+        tensor was computed with."""
+        return _version(self.column_scale) == self._scale_version
 
     def unpack(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """The stored values, contiguous, rounded to ``dtype`` (the packed tensor's own by
@@ -227,6 +238,7 @@ def _trusted(values, exponents, features, column_scale, shape, dtype) -> PackedA
     p = PackedActivation.__new__(PackedActivation)
     p.values, p.exponents, p.features = values, exponents, features
     p.shape, p.dtype, p.column_scale = shape, dtype, column_scale
+    p._scale_version = _version(column_scale)
     return p
 
 
@@ -513,6 +525,8 @@ def linear(
         _require_same_device(packed.values, x.device, "linear: packed")
         if packed.shape != tuple(x.shape):
             raise ValueError(f"linear: packed is of shape {packed.shape}, x of {tuple(x.shape)}")
+        if not packed._scale_is_as_packed():
+            raise ValueError("linear: packed's column scale was written to since x was packed")
     if not (torch.is_grad_enabled()
             and any(t is not None and t.requires_grad for t in (x, weight, bias))):
         return F.linear(x, weight, bias)
@@ -527,8 +541,8 @@ def linear(
 # --- modules ------------------------------------------------------------------------------
 
 # A norm's output carries its packed form with it, as (packed, the output's version), so that the
-# linear layers reading it share one copy.  An output that was written to since, or a tensor made
-# from it, does not have it and is packed by the layer.
+# linear layers reading it share one copy.  An output that was written to since, or whose norm's
+# weight was, or a tensor made from it, does not have it and is packed by the layer.
 _CARRIED = "_torchft_amd_packed"
 
 
@@ -550,7 +564,7 @@ class Linear(nn.Linear):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         carried = getattr(x, _CARRIED, None)
-        if carried is not None and carried[1] == x._version:
+        if carried is not None and carried[1] == x._version and carried[0]._scale_is_as_packed():
             return linear(x, self.weight, self.bias, carried[0])
         return linear(x, self.weight, self.bias)
 
