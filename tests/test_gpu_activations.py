@@ -770,6 +770,16 @@ def test_writing_to_a_norms_weight_before_the_layer_behind_it(device):
         A.linear(out.y, lin.weight, packed=out.packed)
 
 
+def test_giving_a_norms_output_other_storage(device):
+    norm, lin = A.RMSNorm(130).to(device), A.Linear(130, 8).to(device)
+    y, g = norm(randn(1, 6, 130).to(device)), randn(2, 6, 8).to(device)
+    kept = y.detach()
+    y.data = randn(5, 6, 130).to(device)  # torch does not count this as a write
+    gw, = torch.autograd.grad((lin(y) * g).sum(), (lin.weight,))
+    assert_bits_equal(gw, A.linear_weight_grad(g, A.pack(y.detach())))
+    assert not torch.equal(kept, y)
+
+
 def test_autocast(device):
     lin = A.Linear(130, 16).to(device)
     x = randn(1, 9, 130).to(device)

@@ -540,10 +540,29 @@ def linear(
 
 # --- modules ------------------------------------------------------------------------------
 
-# A norm's output carries its packed form with it, as (packed, the output's version), so that the
-# linear layers reading it share one copy.  An output that was written to since, or whose norm's
-# weight was, or a tensor made from it, does not have it and is packed by the layer.
+# A norm's output carries its packed form with it, so that the linear layers reading it share one
+# copy.  An output that was written to since or given other storage, or whose norm's weight was
+# written to, or a tensor made from it, does not have it and is packed by the layer.
 _CARRIED = "_torchft_amd_packed"
+
+
+class _Carried(NamedTuple):
+    packed: PackedActivation
+    version: int  # of the output, when it was made
+    address: int
+
+
+def _carry(y: torch.Tensor, packed: PackedActivation) -> None:
+    setattr(y, _CARRIED, _Carried(packed, y._version, y.data_ptr()))
+
+
+def _carried(x: torch.Tensor) -> Optional[PackedActivation]:
+    """x's packed form, where x carries one and it is still x's."""
+    c = getattr(x, _CARRIED, None)
+    if c is None or c.version != x._version or c.address != x.data_ptr() \
+            or not c.packed._scale_is_as_packed():
+        return None
+    return c.packed
 
 
 class RMSNorm(nn.RMSNorm):
@@ -555,7 +574,7 @@ class RMSNorm(nn.RMSNorm):
             raise ValueError(f"RMSNorm over {tuple(self.normalized_shape)} does not fit {tuple(x.shape)}")
         out = rms_norm(x, self.weight, self.eps, residual)
         if out.packed is not None:
-            setattr(out.y, _CARRIED, (out.packed, out.y._version))
+            _carry(out.y, out.packed)
         return out.y if residual is None else (out.y, out.h)
 
 
@@ -563,10 +582,7 @@ class Linear(nn.Linear):
     """``torch.nn.Linear`` that keeps its input in 8 bits for the weight gradient."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        carried = getattr(x, _CARRIED, None)
-        if carried is not None and carried[1] == x._version and carried[0]._scale_is_as_packed():
-            return linear(x, self.weight, self.bias, carried[0])
-        return linear(x, self.weight, self.bias)
+        return linear(x, self.weight, self.bias, _carried(x))
 
 
 def pack_activations(module: nn.Module) -> nn.Module:
