@@ -61,7 +61,7 @@
 extern "C" {
 #endif
 
-#define TFT_ABI_VERSION 7
+#define TFT_ABI_VERSION 8
 #define TFT_MAX_REPLICAS 8 /* replica pointer columns per launch */
 #define TFT_MIN_CHUNK_ELEMS 8192u
 #define TFT_NOALLOC_MAX_TENSORS 4096u /* rows of the built-in table of the allocation-free entry */
@@ -255,6 +255,12 @@ int tft_mt_copy_bytes(const tft_mt_table* table, void* stream);
  * a multiple of 16 bytes, everything else at a multiple of its element size.  The reference
  * has no counterpart of these entries: it leaves activations to torch.
  */
+
+/* Which graph capture `stream` is recorded by: 0 for none, a number of its own for each capture,
+ * UINT64_MAX where that cannot be told.  What is enqueued under a capture exists with the graph's
+ * replays only, and what was enqueued outside of it is not enqueued again by them: a buffer that
+ * belongs to one of the two is not to be read by the other without the caller's say. */
+uint64_t tft_capture_id(void* stream);
 
 /* x [rows, features] -> packed form */
 int tft_pack_e4m3(void* values, void* exponents, const void* x, int64_t rows, int64_t features,

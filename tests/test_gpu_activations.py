@@ -8,7 +8,7 @@ from torch import nn
 
 from helpers import assert_bits_equal
 from oracle import packed_activations as O
-from torchft_amd import PackedActivation, PureDistributedDataParallel
+from torchft_amd import PackedActivation, PureDistributedDataParallel, _native
 from torchft_amd import activations as A
 
 pytestmark = pytest.mark.gpu
@@ -571,6 +571,39 @@ def small_block(dtype, device):
     torch.manual_seed(0)
     return nn.Sequential(nn.RMSNorm(192, eps=1e-5), nn.Linear(192, 320), nn.SiLU(), nn.Linear(320, 192),
                          nn.RMSNorm(192, eps=1e-5), nn.Linear(192, 100, bias=False)).to(device, dtype)
+
+
+def test_a_captured_layer_packs_what_its_replays_read(device):
+    """The graph holds the layer and not the norm: new rows are written into the norm's output."""
+    norm, lin = A.RMSNorm(130).to(device), A.Linear(130, 8).to(device)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        lin(norm(randn(1, 6, 130).to(device)))
+    torch.cuda.current_stream().wait_stream(side)
+    y = norm(randn(1, 6, 130).to(device))
+    assert _native.lib().tft_capture_id(torch.cuda.current_stream().cuda_stream) == 0
+    kept, ids = [], []
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            out = lin(y)
+            z = norm(y)
+            again = lin(z)  # the graph's own norm packs for this one
+            ids.append(_native.lib().tft_capture_id(torch.cuda.current_stream().cuda_stream))
+            kept.append((out.grad_fn.saved_tensors[1], again.grad_fn.saved_tensors[1]))
+            assert kept[-1][1].data_ptr() == getattr(z, A._CARRIED).packed.values.data_ptr()
+            del out, z, again
+    assert 0 not in ids and ids[0] != ids[1] and A._UNKNOWN_CAPTURE not in ids
+    for k in range(3):
+        with torch.no_grad():
+            y.copy_(randn(k + 7, 6, 130))
+        for graph, (values, normed) in zip(graphs, kept):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert_bits_equal(values.view(torch.uint8), A.pack(y.detach()).values.view(torch.uint8))
+            assert_bits_equal(normed.view(torch.uint8),
+                              A.rms_norm_forward(y.detach(), norm.weight)[2].values.view(torch.uint8))
 
 
 def test_captured_steps_replay(device):

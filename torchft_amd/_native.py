@@ -18,7 +18,7 @@ import torch  # noqa: F401  (must precede loading the library, see module docstr
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libtorchft_amd.so"
 
-ABI_VERSION = 7
+ABI_VERSION = 8
 MAX_REPLICAS = 8
 MIN_CHUNK_ELEMS = 8192
 MIN_CHUNK_BYTES = 16384  # tft_mt_copy_bytes counts bytes
@@ -88,6 +88,7 @@ SIGNATURES = {
     "tft_mt_outer_sgd_of_sum": (c_int, [POINTER(MtTable), c_uint32, c_int, POINTER(SgdParams), c_void_p]),
     "tft_mt_copy_bytes": (c_int, [POINTER(MtTable), c_void_p]),
     "tft_probe_rw_pair": (c_int, [c_void_p, c_void_p, c_uint64, c_void_p]),
+    "tft_capture_id": (c_uint64, [c_void_p]),
     "tft_pack_e4m3": (
         c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]
     ),

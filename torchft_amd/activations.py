@@ -542,7 +542,9 @@ def linear(
 
 # A norm's output carries its packed form with it, so that the linear layers reading it share one
 # copy.  An output that was written to since or given other storage, or whose norm's weight was
-# written to, or a tensor made from it, does not have it and is packed by the layer.
+# written to, or a tensor made from it, does not have it and is packed by the layer.  Neither is the
+# form of an output used by a graph capture that the norm was not part of: the replays would read
+# rows that nobody packs again.
 _CARRIED = "_torchft_amd_packed"
 
 
@@ -550,10 +552,18 @@ class _Carried(NamedTuple):
     packed: PackedActivation
     version: int  # of the output, when it was made
     address: int
+    capture: int  # the graph capture that it was made under
+
+
+_UNKNOWN_CAPTURE = (1 << 64) - 1
+
+
+def _capture(device: torch.device) -> int:
+    return _native.lib().tft_capture_id(_raw_stream(device.index))
 
 
 def _carry(y: torch.Tensor, packed: PackedActivation) -> None:
-    setattr(y, _CARRIED, _Carried(packed, y._version, y.data_ptr()))
+    setattr(y, _CARRIED, _Carried(packed, y._version, y.data_ptr(), _capture(y.device)))
 
 
 def _carried(x: torch.Tensor) -> Optional[PackedActivation]:
@@ -562,7 +572,8 @@ def _carried(x: torch.Tensor) -> Optional[PackedActivation]:
     if c is None or c.version != x._version or c.address != x.data_ptr() \
             or not c.packed._scale_is_as_packed():
         return None
-    return c.packed
+    capture = _capture(x.device)
+    return c.packed if capture == c.capture and capture != _UNKNOWN_CAPTURE else None
 
 
 class RMSNorm(nn.RMSNorm):

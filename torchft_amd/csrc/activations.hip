@@ -1472,6 +1472,16 @@ int launch_wgrad(const char* what, const WgradArgs& a, const WgradPlan& p, const
 
 extern "C" {
 
+uint64_t tft_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &id) != hipSuccess) {
+    (void)hipGetLastError();  // not for the next caller who asks
+    return ~0ull;
+  }
+  return status == hipStreamCaptureStatusNone ? 0 : status == hipStreamCaptureStatusActive ? id + 1 : ~0ull;
+}
+
 int tft_pack_e4m3(void* values, void* exponents, const void* x, int64_t rows, int64_t features,
                   int64_t x_row_stride, int64_t pitch, int dtype, void* stream) {
   static const char* what = "tft_pack_e4m3";
