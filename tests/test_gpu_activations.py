@@ -813,6 +813,32 @@ def test_giving_a_norms_output_other_storage(device):
     assert not torch.equal(kept, y)
 
 
+def test_packed_rows_outlive_the_stream_that_reads_them(device):
+    """A layer on another stream than its norm's: after y.record_stream, as torch asks, the packed
+    rows behind y are not handed out again while that stream may still read them."""
+    norm, lin = A.RMSNorm(4096).to(device), A.Linear(4096, 8).to(device)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        lin(norm(torch.ones(64, 4096, device=device)))
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    y = norm(torch.ones(8192, 4096, device=device))
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        out = lin(y)
+    y.record_stream(side)
+    packed = getattr(y, A._CARRIED).packed
+    kept = packed.values.data_ptr()
+    assert out.grad_fn.saved_tensors[1].data_ptr() == kept
+    del y, out, packed
+    fresh = [torch.empty(8192, 4096, dtype=torch.uint8, device=device) for _ in range(3)]
+    assert not side.query()  # it is still asleep
+    assert kept not in [t.data_ptr() for t in fresh]
+    torch.cuda.synchronize()
+
+
 def test_autocast(device):
     lin = A.Linear(130, 16).to(device)
     x = randn(1, 9, 130).to(device)

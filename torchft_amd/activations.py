@@ -212,6 +212,12 @@ class PackedActivation:
     def nbytes(self) -> int:
         return self.values.numel() + self.exponents.numel()
 
+    def record_stream(self, stream: "torch.cuda.Stream") -> None:
+        """``torch.Tensor.record_stream`` of the two buffers: for a packed form that another stream
+        than the one it was made on reads."""
+        self.values.record_stream(stream)
+        self.exponents.record_stream(stream)
+
     def _scale_is_as_packed(self) -> bool:
         """Whether the column scale (a norm's live weight) is still the one that the packed
         tensor was computed with."""
@@ -456,7 +462,8 @@ def rms_norm(
 ) -> NormOutput:
     """Differentiable root-mean-square norm of h = x + residual: (y, h, packed).  ``packed`` is
     what the backward pass keeps, and what :func:`linear` takes for a layer that reads y; it is
-    None where nothing needs a gradient, and nothing is packed then."""
+    None where nothing needs a gradient, and nothing is packed then.  Its buffers belong to the
+    current stream: a layer on another one needs ``packed.record_stream`` as it needs y's."""
     x = _as_rows(x)
     residual = None if residual is None else _as_rows(residual)
     if not (torch.is_grad_enabled()
@@ -553,17 +560,16 @@ class _Carried(NamedTuple):
     version: int  # of the output, when it was made
     address: int
     capture: int  # the graph capture that it was made under
+    stream: int
 
 
 _UNKNOWN_CAPTURE = (1 << 64) - 1
 
 
-def _capture(device: torch.device) -> int:
-    return _native.lib().tft_capture_id(_raw_stream(device.index))
-
-
 def _carry(y: torch.Tensor, packed: PackedActivation) -> None:
-    setattr(y, _CARRIED, _Carried(packed, y._version, y.data_ptr(), _capture(y.device)))
+    stream = _raw_stream(y.device.index)
+    capture = _native.lib().tft_capture_id(stream)
+    setattr(y, _CARRIED, _Carried(packed, y._version, y.data_ptr(), capture, stream))
 
 
 def _carried(x: torch.Tensor) -> Optional[PackedActivation]:
@@ -572,8 +578,13 @@ def _carried(x: torch.Tensor) -> Optional[PackedActivation]:
     if c is None or c.version != x._version or c.address != x.data_ptr() \
             or not c.packed._scale_is_as_packed():
         return None
-    capture = _capture(x.device)
-    return c.packed if capture == c.capture and capture != _UNKNOWN_CAPTURE else None
+    stream = _raw_stream(x.device.index)
+    capture = _native.lib().tft_capture_id(stream)
+    if capture != c.capture or capture == _UNKNOWN_CAPTURE:
+        return None
+    if stream != c.stream:  # the caller has seen to x; nobody but us knows of what lies behind it
+        c.packed.record_stream(torch.cuda.current_stream(x.device))
+    return c.packed
 
 
 class RMSNorm(nn.RMSNorm):
