@@ -1,5 +1,6 @@
 """Packed activations on the GPU against the 64-bit checker."""
 
+import io
 import math
 
 import pytest
@@ -724,6 +725,84 @@ def test_packed_norm_output_is_shared_by_the_layers_behind_it(device):
         y.mul_(2.0)  # written to since: the layer packs what it sees
     gw, = torch.autograd.grad((a(y) * ga).sum(), (a.weight,))
     assert_bits_equal(gw, A.linear_weight_grad(ga, A.pack(y.detach())))
+
+
+@pytest.mark.parametrize("autocast", [False, True])
+def test_layers_that_read_one_activation_keep_one_copy(device, autocast):
+    """Query, key and value projections behind a norm that is not ours, as one after another and as
+    a whole: the bytes that they keep, their gradients, and what is left once they are gone."""
+    rows, features = 64, 1024
+    ln = nn.LayerNorm(features).to(device)
+    layers = [A.Linear(features, 16).to(device) for _ in range(3)]
+    y = ln(randn(1, rows, features).to(device))
+    grads = [randn(k, rows, 16).to(device) for k in range(3)]
+    with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+        [layer(y) for layer in layers]  # whatever the products allocate once
+        before = torch.cuda.memory_allocated()
+        outs = [layer(y) for layer in layers]
+        kept = {o.grad_fn.saved_tensors[1].data_ptr() for o in outs}
+        nothing = [nn.functional.linear(y.detach(), layer.weight.detach()) for layer in layers]
+        assert len(kept) == 1
+    if not autocast:  # the outputs, and their values and exponents
+        assert torch.cuda.memory_allocated() - before <= 6 * rows * 16 * 4 + rows * (features + features // 128)
+    del nothing
+    got = torch.autograd.grad([(o * g).sum() for o, g in zip(outs, grads)], [layer.weight for layer in layers])
+    cast = y.detach().bfloat16() if autocast else y.detach()
+    for gw, g in zip(got, grads):
+        assert_bits_equal(gw, A.linear_weight_grad(g.to(cast.dtype), A.pack(cast)).float())
+    del outs, got, gw
+    weak = getattr(y, A._SHARED)
+    assert weak.values() is None and weak.exponents() is None
+    with torch.no_grad():
+        y.mul_(2.0)
+    first = layers[0](y)
+    with torch.no_grad():
+        y.mul_(2.0)  # the first layer's rows are no longer y's
+    second = layers[1](y)
+    gw, = torch.autograd.grad((second * grads[1]).sum(), (layers[1].weight,))
+    assert_bits_equal(gw, A.linear_weight_grad(grads[1], A.pack(y.detach())))
+    gw, = torch.autograd.grad((first * grads[0]).sum(), (layers[0].weight,))
+    assert_bits_equal(gw, A.linear_weight_grad(grads[0], A.pack(y.detach() / 2)))
+
+
+def test_layers_on_other_streams_pack_for_themselves(device):
+    """Nothing makes the second stream wait for what the first one packed."""
+    layers = [A.Linear(256, 16).to(device) for _ in range(2)]
+    y = torch.relu(randn(1, 40, 256).to(device).requires_grad_())
+    first = layers[0](y)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = layers[1](y)
+    a, b = first.grad_fn.saved_tensors[1], second.grad_fn.saved_tensors[1]
+    torch.cuda.synchronize()
+    assert a.data_ptr() != b.data_ptr()
+    assert_bits_equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_a_shared_activation_saves_and_loads_as_a_tensor(device):
+    y = torch.relu(randn(1, 40, 256).to(device).requires_grad_())
+    layer = A.Linear(256, 16).to(device)
+    out = layer(y)
+    file = io.BytesIO()
+    torch.save(y, file)
+    file.seek(0)
+    again = torch.load(file, weights_only=True)
+    assert torch.equal(again, y)
+    assert_bits_equal(layer(torch.relu(again)), out)
+    assert_bits_equal(layer(again), out)
+
+
+def test_input_buffers_are_packed_by_every_layer(device):
+    """A program's own buffer may be rewritten in ways that torch does not count."""
+    layers = [A.Linear(256, 16).to(device) for _ in range(2)]
+    x = randn(1, 40, 256).to(device)
+    first = layers[0](x)
+    x.data.copy_(randn(2, 40, 256))
+    g = randn(3, 40, 16).to(device)
+    gw, = torch.autograd.grad((layers[1](x) * g).sum(), (layers[1].weight,))
+    assert_bits_equal(gw, A.linear_weight_grad(g, A.pack(x)))
+    del first
 
 
 def test_modules_without_gradients_and_without_rows(device):

@@ -22,11 +22,13 @@ device, never synchronise, and have no CPU path.  The reference has no counterpa
 from __future__ import annotations
 
 import math
+from collections import OrderedDict
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
 from torch import nn
+from torch.utils.weak import TensorWeakRef
 
 from . import _native
 
@@ -520,6 +522,14 @@ def linear(
     """``torch.nn.functional.linear`` that keeps its input in 8 bits.  ``packed`` is x in that form
     where the caller has it (:func:`rms_norm`, or another layer's :func:`pack` of the same x);
     otherwise x is packed here, unless the weight needs no gradient."""
+    return _linear(x, weight, bias, packed, share=False)
+
+
+def _linear(
+    x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], packed: Optional[PackedActivation],
+    share: bool,
+) -> torch.Tensor:
+    given = x
     _require_gpu(x, "linear: x")
     if x.dim() == 0 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"linear: x of shape {tuple(x.shape)} does not fit a weight of {tuple(weight.shape)}")
@@ -537,6 +547,8 @@ def linear(
     if not (torch.is_grad_enabled()
             and any(t is not None and t.requires_grad for t in (x, weight, bias))):
         return F.linear(x, weight, bias)
+    if packed is None and share and given.grad_fn is not None and weight.requires_grad:
+        packed = _shared(given, x)
     return _LinearFunction.apply(
         x, weight, bias,
         None if packed is None else packed.values,
@@ -587,6 +599,45 @@ def _carried(x: torch.Tensor) -> Optional[PackedActivation]:
     return c.packed
 
 
+# Several layers may read an activation that no norm of ours made.  The first of them packs it, and
+# the others find its packed form by weak references on the activation: it lives as long as the
+# backward pass of one of them needs it, and no longer because the activation does.  The same layers
+# have to read it on the same stream: nothing makes another one wait for the packing.  Tensors that
+# autograd did not make are packed by every layer: a program's input buffers are written to in ways
+# that torch does not count (graph replays among them).
+_SHARED = "_torchft_amd_shared"
+
+
+class _Shared(NamedTuple):
+    values: TensorWeakRef
+    exponents: TensorWeakRef
+    dtype: torch.dtype  # what was packed: the activation, or what autocast made of it
+    version: int  # of the activation
+    address: int
+    capture: int
+    stream: int
+
+    def __reduce_ex__(self, protocol: object) -> tuple:  # a saved or copied activation is not packed
+        return OrderedDict, ()
+
+
+def _shared(given: torch.Tensor, x: torch.Tensor) -> Optional[PackedActivation]:
+    """x, which is ``given`` itself or its cast, packed once for all layers that read ``given``."""
+    stream = _raw_stream(given.device.index)
+    capture = _native.lib().tft_capture_id(stream)
+    if capture == _UNKNOWN_CAPTURE:
+        return None
+    now = (x.dtype, given._version, given.data_ptr(), capture, stream)
+    s = getattr(given, _SHARED, None)
+    if type(s) is _Shared and s[2:] == now:
+        values, exponents = s.values(), s.exponents()
+        if values is not None and exponents is not None:
+            return _trusted(values, exponents, x.shape[-1], None, tuple(x.shape), x.dtype)
+    packed = pack(_as_rows(x.detach()))
+    setattr(given, _SHARED, _Shared(TensorWeakRef(packed.values), TensorWeakRef(packed.exponents), *now))
+    return packed
+
+
 class RMSNorm(nn.RMSNorm):
     """``torch.nn.RMSNorm`` over the last dimension that keeps its normalised rows in 8 bits.
     ``forward(x, residual)`` norms h = x + residual and returns (y, h).  The output has x's type."""
@@ -601,10 +652,11 @@ class RMSNorm(nn.RMSNorm):
 
 
 class Linear(nn.Linear):
-    """``torch.nn.Linear`` that keeps its input in 8 bits for the weight gradient."""
+    """``torch.nn.Linear`` that keeps its input in 8 bits for the weight gradient, once for all such
+    layers that read it."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return linear(x, self.weight, self.bias, _carried(x))
+        return _linear(x, self.weight, self.bias, _carried(x), share=True)
 
 
 def pack_activations(module: nn.Module) -> nn.Module:
