@@ -793,6 +793,19 @@ def test_a_shared_activation_saves_and_loads_as_a_tensor(device):
     assert_bits_equal(layer(again), out)
 
 
+def test_a_norms_output_saves_and_loads_as_a_tensor(device):
+    """Its packed rows are not written with it: safe loading would refuse their class."""
+    norm, layer = A.RMSNorm(256).to(device), A.Linear(256, 16).to(device)
+    y = norm(randn(1, 40, 256).to(device))
+    file = io.BytesIO()
+    torch.save(y, file)
+    assert len(file.getvalue()) < 40 * 256 * 4 + 4096
+    file.seek(0)
+    again = torch.load(file, weights_only=True)
+    assert torch.equal(again, y)
+    assert_bits_equal(layer(again), layer(y))
+
+
 def test_input_buffers_are_packed_by_every_layer(device):
     """A program's own buffer may be rewritten in ways that torch does not count."""
     layers = [A.Linear(256, 16).to(device) for _ in range(2)]

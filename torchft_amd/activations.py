@@ -574,6 +574,9 @@ class _Carried(NamedTuple):
     capture: int  # the graph capture that it was made under
     stream: int
 
+    def __reduce_ex__(self, protocol: object) -> tuple:  # a saved or copied output is not packed
+        return OrderedDict, ()
+
 
 _UNKNOWN_CAPTURE = (1 << 64) - 1
 
@@ -587,7 +590,7 @@ def _carry(y: torch.Tensor, packed: PackedActivation) -> None:
 def _carried(x: torch.Tensor) -> Optional[PackedActivation]:
     """x's packed form, where x carries one and it is still x's."""
     c = getattr(x, _CARRIED, None)
-    if c is None or c.version != x._version or c.address != x.data_ptr() \
+    if type(c) is not _Carried or c.version != x._version or c.address != x.data_ptr() \
             or not c.packed._scale_is_as_packed():
         return None
     stream = _raw_stream(x.device.index)
