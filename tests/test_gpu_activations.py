@@ -780,6 +780,34 @@ def test_layers_on_other_streams_pack_for_themselves(device):
     assert_bits_equal(a.view(torch.uint8), b.view(torch.uint8))
 
 
+def test_views_of_a_norms_output_share_its_rows(device):
+    norm, layer = A.RMSNorm(256).to(device), A.Linear(256, 16).to(device)
+    y = norm(randn(1, 2, 20, 256).to(device))
+    kept = getattr(y, A._CARRIED).packed.values
+    g = randn(2, 40, 16).to(device)
+    for whole in (y.view(-1, 256), y.flatten(0, 1), y.unsqueeze(0), y.view(4, 10, 256)):
+        out = layer(whole)
+        assert out.grad_fn.saved_tensors[1].data_ptr() == kept.data_ptr()
+        gw, = torch.autograd.grad((out.view(40, 16) * g).sum(), (layer.weight,))
+        assert_bits_equal(gw, A.linear_weight_grad(g, getattr(y, A._CARRIED).packed))
+    square = A.RMSNorm(16).to(device)(randn(1, 16, 16).to(device))
+    narrow = A.Linear(16, 8).to(device)
+    for part in (square[:15], square[1:], square.t(), square.view(16, 1, 16).expand(16, 2, 16), square.view(256, 1),
+                 square.view(8, 32)):  # other rows, another order, rows twice, other rows' ends
+        lin = narrow if part.shape[-1] == 16 else A.Linear(part.shape[-1], 8).to(device)
+        out = lin(part)
+        g = randn(3, *out.shape).to(device)
+        gw, = torch.autograd.grad((out * g).sum(), (lin.weight,))
+        rows = part.detach().reshape(-1, part.shape[-1]).contiguous()
+        assert_bits_equal(gw, A.linear_weight_grad(g.reshape(-1, 8), A.pack(rows)))
+    flat = y.view(-1, 256)
+    with torch.no_grad():
+        flat.mul_(2.0)  # a write to one is a write to all
+    for t in (flat, y.view(-1, 256)):
+        gw, = torch.autograd.grad((layer(t) * randn(2, 40, 16).to(device)).sum(), (layer.weight,))
+        assert_bits_equal(gw, A.linear_weight_grad(randn(2, 40, 16).to(device), A.pack(t.detach())))
+
+
 def test_a_shared_activation_saves_and_loads_as_a_tensor(device):
     y = torch.relu(randn(1, 40, 256).to(device).requires_grad_())
     layer = A.Linear(256, 16).to(device)

@@ -561,8 +561,8 @@ def _linear(
 
 # A norm's output carries its packed form with it, so that the linear layers reading it share one
 # copy.  An output that was written to since or given other storage, or whose norm's weight was
-# written to, or a tensor made from it, does not have it and is packed by the layer.  Neither is the
-# form of an output used by a graph capture that the norm was not part of: the replays would read
+# written to, or a tensor made from it (all its rows in another shape apart), does not have it and is
+# packed by the layer.  Neither is the form of an output used by a graph capture that the norm was not part of: the replays would read
 # rows that nobody packs again.
 _CARRIED = "_torchft_amd_packed"
 
@@ -588,8 +588,15 @@ def _carry(y: torch.Tensor, packed: PackedActivation) -> None:
 
 
 def _carried(x: torch.Tensor) -> Optional[PackedActivation]:
-    """x's packed form, where x carries one and it is still x's."""
+    """x's packed form, where x carries one and it is still x's, or where x is a view of all rows of
+    a tensor that does."""
     c = getattr(x, _CARRIED, None)
+    if c is None and torch.is_grad_enabled() and x._is_view():
+        whole = x._base
+        c = getattr(whole, _CARRIED, None)
+        if c is not None and not (x.dim() and x.shape[-1:] == whole.shape[-1:] and x.numel() == whole.numel()
+                                  and x.dtype == whole.dtype and x.is_contiguous() and whole.is_contiguous()):
+            return None
     if type(c) is not _Carried or c.version != x._version or c.address != x.data_ptr() \
             or not c.packed._scale_is_as_packed():
         return None
@@ -599,6 +606,9 @@ def _carried(x: torch.Tensor) -> Optional[PackedActivation]:
         return None
     if stream != c.stream:  # the caller has seen to x; nobody but us knows of what lies behind it
         c.packed.record_stream(torch.cuda.current_stream(x.device))
+    if c.packed.shape != tuple(x.shape):
+        p = c.packed
+        return _trusted(p.values, p.exponents, p.features, p.column_scale, tuple(x.shape), p.dtype)
     return c.packed
 
 
