@@ -5,11 +5,14 @@ import copy
 import ctypes
 import math
 import pickle
+import subprocess
+import sys
 
 import pytest
 import torch
 from torch import nn
 
+from conftest import REPO_ROOT
 from oracle import packed_activations as O
 from torchft_amd import PackedActivation, PureDistributedDataParallel, _native, pack_activations
 from torchft_amd import activations as A
@@ -272,6 +275,17 @@ def test_weight_gradients_of_more_tiles_than_a_launch_holds_are_refused():
 
 
 # --- modules ------------------------------------------------------------------------------------
+
+
+def test_imports_under_a_torch_without_gpu_support():
+    """Such a build lacks the names that ask for the current stream and device."""
+    code = ("import torch\n"
+            "for name in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):\n"
+            "    delattr(torch._C, name)\n"
+            "import torchft_amd\n"
+            "torchft_amd.pack_activations(torch.nn.Linear(2, 2))\n")
+    done = subprocess.run([sys.executable, "-c", code], cwd=REPO_ROOT, capture_output=True, text=True, timeout=110)
+    assert done.returncode == 0, done.stderr
 
 
 class Odd(nn.Linear):

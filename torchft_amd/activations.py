@@ -50,8 +50,13 @@ def _dtype_code(dtype: torch.dtype, what: str) -> int:
         raise TypeError(f"{what}: float32, bfloat16 and float16 are supported, got {dtype}") from None
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# Looked up when called: a build of torch without GPU support has neither, and imports this.
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()
 
 
 def _launch(name: str, device: torch.device, *args: object) -> None:
