@@ -230,6 +230,32 @@ def test_norm_without_eps_is_torchs(device, dtype, size):
     assert_bits_equal(A.rms_norm_forward(x.to(device))[0], after)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("weight_dtype", DTYPES)
+def test_norm_module_takes_weights_of_every_type(device, dtype, weight_dtype):
+    norm = nn.RMSNorm(130, eps=1e-5).to(device, weight_dtype)
+    with torch.no_grad():
+        norm.weight.copy_(1 + 0.3 * randn(2, 130))
+    x = randn(1, 6, 130, dtype=dtype)
+    want = O.rms_norm(x, norm.weight.detach().cpu(), 1e-5)[0]
+    tol = want.abs() * (45 / 2 + 5) * 2.0 ** -24 + rounding(want, dtype) * (1 + 2.0 ** -10)
+    before = norm(x.to(device))
+    after = A.pack_activations(norm)(x.to(device))
+    assert before.dtype == after.dtype == dtype
+    assert_within(after, want, tol, "y")
+    with torch.no_grad():
+        assert_bits_equal(norm(x.to(device)), after)
+    g = randn(3, 6, 130, dtype=dtype)
+    gw, = torch.autograd.grad(after, (norm.weight,), g.to(device))
+    packed = getattr(after, A._CARRIED).packed
+    n = O.unpack(*codes_of(packed))
+    _, want = O.rms_norm_backward(g, n, torch.ones(6), None)
+    # six products added in fp32, rounded to fp32 and then to the weight's type
+    tol = (g.double() * n).abs().sum(dim=0) * 8 * 2.0 ** -24 + rounding(want, weight_dtype) * (1 + 2.0 ** -10)
+    assert gw.dtype == weight_dtype
+    assert_within(gw, want, tol, "grad_weight")
+
+
 def test_norm_of_rows_of_zeros_and_nan(device):
     x = randn(1, 4, 200)
     x[1] = 0.0

@@ -469,10 +469,13 @@ def rms_norm(
 ) -> NormOutput:
     """Differentiable root-mean-square norm of h = x + residual: (y, h, packed).  ``packed`` is
     what the backward pass keeps, and what :func:`linear` takes for a layer that reads y; it is
-    None where nothing needs a gradient, and nothing is packed then.  Its buffers belong to the
+    None where nothing needs a gradient, and nothing is packed then.  y and h have x's type; a weight
+    of a third type takes part as its fp32 numbers, as in torch's norm.  ``packed``'s buffers belong to the
     current stream: a layer on another one needs ``packed.record_stream`` as it needs y's."""
     x = _as_rows(x)
     residual = None if residual is None else _as_rows(residual)
+    if weight is not None and weight.dtype != x.dtype and weight.dtype in (torch.bfloat16, torch.float16):
+        weight = weight.float()
     if not (torch.is_grad_enabled()
             and any(t is not None and t.requires_grad for t in (x, residual, weight))):
         y, h, _, _ = rms_norm_forward(x, weight, eps, residual, pack=False)
