@@ -999,6 +999,16 @@ def test_autocast(device):
     assert torch.equal(lin.weight.grad, want.float())
 
 
+def test_autocast_leaves_64_bits_alone(device):
+    x = randn(1, 3, 8).to(device)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert nn.functional.linear(x.double(), x.double()).dtype == torch.float64
+        with pytest.raises(TypeError, match="float64"):
+            A.Linear(8, 4).to(device).double()(x.double())
+        with pytest.raises(TypeError, match="float64"):
+            A.linear(x.double(), randn(2, 4, 8).to(device))
+
+
 class Averaging:
     """A manager whose all-reduce halves the gradient, as two participants with one idle would."""
 

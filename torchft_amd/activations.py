@@ -543,8 +543,8 @@ def _linear(
         raise ValueError(f"linear: x of shape {tuple(x.shape)} does not fit a weight of {tuple(weight.shape)}")
     if torch.is_autocast_enabled("cuda"):
         dtype = torch.get_autocast_dtype("cuda")
-        x, weight = x.to(dtype), weight.to(dtype)
-        bias = None if bias is None else bias.to(dtype)
+        # as torch: 64-bit tensors are left as they are (and refused below)
+        x, weight, bias = (t if t is None or t.dtype == torch.float64 else t.to(dtype) for t in (x, weight, bias))
     _dtype_code(x.dtype, "linear")
     if packed is not None:
         _require_same_device(packed.values, x.device, "linear: packed")
