@@ -85,3 +85,22 @@ def rms_norm_backward(grad_y, n, rstd, weight, grad_h=None):
 def linear_weight_grad(grad_out, x, column_scale: Optional[torch.Tensor] = None):
     out = grad_out.double().t() @ x.double()
     return out if column_scale is None else out * column_scale.double()
+
+
+def bf16_parts(v: torch.Tensor, parts: int) -> torch.Tensor:
+    """What ``parts`` bf16 numbers, each cut off from what the ones before leave, add up to."""
+    left, total = v.float(), torch.zeros(v.shape, dtype=torch.float64)
+    for _ in range(parts):
+        cut = (left.view(torch.int32) & -65536).view(torch.float32)
+        total += cut.double()
+        left = left - cut
+    return total
+
+
+def weight_grad_bound(grad_out, x, parts: int):
+    """How far sums in fp32 may be off, products being exact.  Matrix instructions of 16 tokens align
+    what they add to the largest of it: every product and the sum so far may lose a step of 2^-23.
+    Tokens of zeros add nothing; pieces of the sum are joined by at most a rounding each."""
+    groups = -(-grad_out.shape[0] // 16)
+    steps = parts * (grad_out.shape[0] + groups) + groups
+    return linear_weight_grad(grad_out.abs(), x.abs()) * steps * 2.0 ** -23

@@ -89,6 +89,20 @@ def test_checkers_gradients_are_differences():
         assert abs((loss(x, r, w + d) - loss(x, r, w - d)) / (2 * step) - float(gw[j])) < 1e-7
 
 
+@pytest.mark.parametrize("dtype,parts", [(torch.float32, 3), (torch.float16, 2)])
+@pytest.mark.parametrize("rows", [1, 3, 8])
+def test_bound_of_the_weight_gradient_tells_a_missing_part(dtype, parts, rows):
+    """A gradient cut into one bf16 part too few is outside of the bound that the GPU's is held to."""
+    g = torch.Generator().manual_seed(rows)
+    d = torch.randn(rows, 40, generator=g).to(dtype)
+    x = O.unpack(*O.pack(torch.randn(rows, 30, generator=g)))
+    want, bound = O.linear_weight_grad(d, x), O.weight_grad_bound(d, x, parts)
+    assert torch.equal(O.bf16_parts(d, parts), d.double())
+    short = O.linear_weight_grad(O.bf16_parts(d, parts - 1), x)
+    assert ((short - want).abs() > bound).double().mean() > 0.5
+    assert ((d.float().t() @ x.float()).double() - want).abs().le(bound).all()
+
+
 # --- refusals -----------------------------------------------------------------------------------
 
 

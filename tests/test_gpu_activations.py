@@ -399,6 +399,49 @@ def test_weight_gradient_of_large_layers(device, rows, out_features, features, d
     big_wgrad(device, rows, out_features, features, dtype)
 
 
+def plan_of(device, rows, out_features, features, dtype):
+    """Pieces' workspace of a weight gradient whose rows are read as they lie."""
+    d = torch.empty(16, device=device, dtype=dtype)
+    return _native.lib().tft_linear_weight_grad_workspace(d.data_ptr(), rows, out_features, features, out_features,
+                                                          (features + 15) // 16 * 16, A._DTYPES[dtype])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,out_features,features,cut", [
+    (1, 64, 64, False), (65, 136, 144, None), (70, 14336, 4096, None), (300, 4096, 2560, None),
+    (1000, 1000, 768, True), (4096, 1024, 4096, True), (2049, 130, 128, None), (40, 61, 77, False)])
+def test_weight_gradient_keeps_every_bit(device, dtype, rows, out_features, features, cut):
+    """One row of gradients of full significands against powers of two: every output is a product,
+    and exact.  Large and small tiles, whole and cut ones; the row lies in each part of a step."""
+    if cut is not None and out_features % 8 == 0:
+        assert bool(plan_of(device, rows, out_features, features, dtype)) == cut
+    g = torch.Generator().manual_seed(rows)
+    signs = torch.randint(0, 2, (1, features), generator=g) * 2 - 1
+    x_row = torch.exp2(torch.randint(-6, 7, (1, features), generator=g).float()) * signs
+    bits = torch.randint(0, 1 << 30, (1, out_features), generator=g).double() * 2.0 ** -30 + 1.0  # 1 .. 2
+    small = [] if dtype == torch.float16 else [2.0 ** -104]
+    for at, size in [(0, 0.5), (rows - 1, 1.0), (rows // 2, 2.0 ** -8), *((rows // 3, s) for s in small)]:
+        d_row = (bits * size).to(dtype)
+        d = torch.zeros(rows, out_features, dtype=dtype, device=device)
+        x = torch.zeros(rows, features, device=device)
+        d[at], x[at] = d_row[0].to(device), x_row[0].to(device)
+        got = A.linear_weight_grad(d, A.pack(x), dtype=torch.float32)
+        want = d[at].double()[:, None] * x[at].double()  # 24 bits times a power of two
+        assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 2, 3, 8, 17, 40])
+def test_weight_gradient_of_few_rows(device, dtype, rows):
+    """Bounds tight enough to tell a missing part of the gradient from a rounding."""
+    d = randn(rows, rows, 72).to(dtype)
+    p = A.pack(randn(rows + 1, rows, 130).to(device))
+    n = O.unpack(*codes_of(p))
+    got = A.linear_weight_grad(d.to(device), p, dtype=torch.float32)
+    want = O.linear_weight_grad(d, n)
+    assert_within(got, want, O.weight_grad_bound(d, n, PARTS[dtype]) + want.abs() * 2.0 ** -24, "weight gradient")
+
+
 @pytest.mark.parametrize("dtype,stride", [(torch.bfloat16, 1 << 24), (torch.float16, 1 << 24), (torch.float32, 1 << 23),
                                           (torch.bfloat16, (1 << 24) - 8), (torch.float32, (1 << 23) + 1)])
 def test_weight_gradient_of_rows_far_apart(device, dtype, stride):

@@ -383,7 +383,7 @@ def linear_weight_grad(
 ) -> torch.Tensor:
     """grad_out^T . packed of [out_features, features]: a linear layer's weight gradient from its
     packed input.  Sums are held in fp32 and rounded once to ``dtype`` (grad_out's by default);
-    fp16 and fp32 gradients lose no bits."""
+    fp16 gradients lose no bits, nor do fp32 ones above 2^-110 (what lies under 2^-133 is cut off)."""
     rows, out_features, stride = _matrix(grad_out, "linear_weight_grad: grad_out")
     code = _dtype_code(grad_out.dtype, "linear_weight_grad")
     dtype = grad_out.dtype if dtype is None else dtype

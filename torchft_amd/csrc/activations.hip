@@ -718,7 +718,8 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const void* x, float* p
 // ---------------------------------------------------------------------------
 // The products run on the bf16 matrix cores.  X is exact in bf16, and D is split into bf16 parts
 // that add up to it exactly while it goes into LDS: one part for bf16, two for fp16 (11 bits),
-// three for fp32 (24 bits).  Every part is multiplied with the same X.
+// three for fp32 (24 bits; the matrix cores take bf16's subnormal numbers, so that only bits under
+// 2^-133 are lost).  Every part is multiplied with the same X.
 template <typename T>
 struct Parts;
 template <>
