@@ -1112,3 +1112,97 @@ def test_wrapped_model_trains_on_packed_activations(device, dtype, near, wrapper
     for (name, p), q in zip(model.named_parameters(), plain.parameters()):
         off = float((2 * p.grad - q.grad).norm() / q.grad.norm())
         assert off < near, f"{name}: {off}"
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+@pytest.mark.parametrize("autocast", [False, True])
+def test_checkpointed_layers(device, reentrant, autocast):
+    """The second forward pass packs what the first one did: the gradients are the same bits."""
+    from torch.utils.checkpoint import checkpoint
+
+    torch.manual_seed(1)
+    before, block = nn.LayerNorm(192).to(device), A.pack_activations(small_block(torch.float32, device))
+    q, k = A.Linear(192, 100).to(device), A.Linear(192, 100).to(device)
+    params = [before.weight, *block.parameters(), q.weight, k.weight]
+
+    def part(x):  # an input that several layers read, and one behind a norm
+        return block(x) + q(x) * k(x)
+
+    def step(run):
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+            out = run(before(randn(2, 33, 192).to(device)))
+        return out.detach(), torch.autograd.grad((out.float() * randn(3, 33, 100).to(device)).sum(), params)
+
+    out, want = step(part)
+    if reentrant:
+        for p in params:
+            p.grad = None
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+            again = checkpoint(part, before(randn(2, 33, 192).to(device)), use_reentrant=True)
+        (again.float() * randn(3, 33, 100).to(device)).sum().backward()
+        got = [p.grad for p in params]
+    else:
+        again, got = step(lambda x: checkpoint(part, x, use_reentrant=False))
+    assert_bits_equal(again, out)
+    for a, b in zip(got, want):
+        assert_bits_equal(a, b)
+
+
+@pytest.mark.parametrize("outer_step", [False, True])
+def test_converted_model_under_localsgd_and_diloco(device, outer_step):
+    """Two replicas, a sync behind every step: the parameters that the kernels write, the norm's
+    weights among them, are those that the next step's gradients are made with."""
+    import copy
+
+    from oracle import replica_sync as sync
+    from test_gpu_api import cpu, peer_world
+    from torch import optim
+    from torchft_amd import DiLoCo, LocalSGD, Manager, ProcessGroupLocalReplicas, StaticQuorum
+
+    torch.manual_seed(2)
+    plain = nn.Sequential(nn.RMSNorm(192), nn.Linear(192, 64), nn.SiLU(), nn.Linear(64, 10)).to(device)
+    model = A.pack_activations(copy.deepcopy(plain))
+    peers, lookup = peer_world(model, 2)
+    g = torch.Generator().manual_seed(7)
+    for q in peers[0].parameters():
+        q.data.add_((torch.randn(q.shape, generator=g) * 1e-2).to(device))
+    pg = ProcessGroupLocalReplicas(rank=0, world_size=2, peer_lookup=lookup)
+    manager = Manager(pg=pg, load_state_dict=None, state_dict=None, min_replica_size=2, use_async_quorum=False,
+                      quorum_client=StaticQuorum(0, 2))
+    inner = optim.SGD(model.parameters(), lr=0.1)
+    if outer_step:
+        wrapped = DiLoCo(manager, model, inner, optim.SGD(model.parameters(), lr=0.7, momentum=0.9, nesterov=True),
+                         sync_every=1)
+    else:
+        wrapped = LocalSGD(manager, model, inner, sync_every=1)
+    seen = {}
+    with wrapped:
+        perform = wrapped._perform_sync
+
+        def recording():
+            seen["local"] = cpu(p.data for p in model.parameters())
+            perform()
+
+        wrapped._perform_sync = recording
+        backup, bufs = cpu(wrapped._backup_parameters.values()), None
+        for step in range(3):
+            fresh = copy.deepcopy(model)
+            x, t = randn(step, 40, 192).to(device), randn(step + 9, 40, 10).to(device)
+            inner.zero_grad()
+            (model(x) * t).sum().backward()
+            (fresh(x) * t).sum().backward()
+            for p, q in zip(model.parameters(), fresh.parameters()):
+                assert_bits_equal(p.grad, q.grad)
+            inner.step()  # the sync runs behind it
+            replicas = [seen["local"], cpu(q.data for q in peers[0].parameters())]
+            if outer_step:
+                want = sync.diloco_perform_sync(replicas, backup, bufs, [True] * 2, 2, True, lr=0.7, momentum=0.9,
+                                                nesterov=True)
+                bufs = want["momentum"]
+            else:
+                want = sync.localsgd_perform_sync(replicas, backup, [True, True], 2, True)
+            backup = want["backup"] if outer_step else want["params"]
+            for p, w in zip(model.parameters(), want["params"]):
+                assert_bits_equal(p.data, w)
+    assert manager.current_step() == 3
+    manager.shutdown(wait=False)
