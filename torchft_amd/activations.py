@@ -50,13 +50,9 @@ def _dtype_code(dtype: torch.dtype, what: str) -> int:
         raise TypeError(f"{what}: float32, bfloat16 and float16 are supported, got {dtype}") from None
 
 
-# Looked up when called: a build of torch without GPU support has neither, and imports this.
 def _raw_stream(index: int) -> int:
+    # looked up when called, as below: a build of torch without GPU support lacks it, and imports this
     return torch._C._cuda_getCurrentRawStream(index)
-
-
-def _current_device() -> int:
-    return torch._C._cuda_getDevice()
 
 
 def _launch(name: str, device: torch.device, *args: object) -> None:
@@ -65,8 +61,8 @@ def _launch(name: str, device: torch.device, *args: object) -> None:
     asked for without an object around it (1.2 and 1.8 microseconds of 10)."""
     index = device.index
     fn = getattr(_native.lib(), name)
-    if _current_device() == index:
-        rc = fn(*args, _raw_stream(index))
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
             rc = fn(*args, _raw_stream(index))
@@ -654,7 +650,7 @@ def _shared(given: torch.Tensor, x: torch.Tensor) -> Optional[PackedActivation]:
         values, exponents = s.values(), s.exponents()
         if values is not None and exponents is not None:
             return _trusted(values, exponents, x.shape[-1], None, tuple(x.shape), x.dtype)
-    packed = pack(_as_rows(x.detach()))
+    packed = pack(_as_rows(x))
     setattr(given, _SHARED, _Shared(TensorWeakRef(packed.values), TensorWeakRef(packed.exponents), *now))
     return packed
 
