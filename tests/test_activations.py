@@ -159,6 +159,28 @@ def test_packed_form_is_checked():
     assert (p.rows, p.shape, p.dtype, p.nbytes) == (2, (2, 130), torch.bfloat16, 2 * 146)
 
 
+def test_packed_form_is_copied_and_pickled():
+    """A copy's scale counts its writes from nought; one that was void stays void."""
+    def form():
+        scale = torch.zeros(130).add_(1.0)
+        return A._trusted(torch.ones(2, 144, dtype=torch.uint8), torch.ones(2, 2, dtype=torch.uint8), 130, scale,
+                          (1, 2, 130), torch.float16)
+
+    for copied in (copy.copy, copy.deepcopy, lambda p: pickle.loads(pickle.dumps(p))):
+        p = form()
+        q = copied(p)
+        assert q._scale_is_as_packed() and (q.shape, q.dtype, q.features) == (p.shape, p.dtype, p.features)
+        assert torch.equal(q.values, p.values) and torch.equal(q.exponents, p.exponents)
+        q.column_scale.mul_(2.0)
+        assert not q._scale_is_as_packed()
+        p = form()
+        p.column_scale.mul_(2.0)
+        assert not copied(p)._scale_is_as_packed()
+        p.column_scale = None
+        p._scale_version = None
+        assert copied(p)._scale_is_as_packed() and copied(p).column_scale is None
+
+
 def test_norm_refuses():
     x = gpu(torch.zeros(2, 16, dtype=torch.bfloat16))
     with pytest.raises(ValueError, match="16 consecutive"):

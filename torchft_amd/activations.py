@@ -226,6 +226,10 @@ class PackedActivation:
         tensor was computed with."""
         return _version(self.column_scale) == self._scale_version
 
+    def __reduce__(self) -> tuple:  # a copy's column scale counts its writes anew
+        return _restored, (self.values, self.exponents, self.features, self.column_scale, self.shape, self.dtype,
+                           self._scale_is_as_packed())
+
     def unpack(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """The stored values, contiguous, rounded to ``dtype`` (the packed tensor's own by
         default; without a column scale they are exact in bf16 and fp32)."""
@@ -248,6 +252,13 @@ def _trusted(values, exponents, features, column_scale, shape, dtype) -> PackedA
     p.values, p.exponents, p.features = values, exponents, features
     p.shape, p.dtype, p.column_scale = shape, dtype, column_scale
     p._scale_version = _version(column_scale)
+    return p
+
+
+def _restored(values, exponents, features, column_scale, shape, dtype, scale_is_as_packed) -> PackedActivation:
+    p = _trusted(values, exponents, features, column_scale, shape, dtype)
+    if not scale_is_as_packed:
+        p._scale_version = -1
     return p
 
 
