@@ -118,6 +118,12 @@ def test_no_cpu_path():
         A.pack([1.0])
 
 
+def test_layer_names_what_is_no_tensor():
+    for x in (None, [1.0], 3):
+        with pytest.raises(TypeError, match="linear: x: expected a tensor"):
+            A.Linear(128, 3)(x)
+
+
 class FakeGpu(torch.Tensor):
     """A CPU tensor that says it is on a GPU: the checks run, nothing is launched."""
 

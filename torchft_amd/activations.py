@@ -553,6 +553,8 @@ def _linear(
         # as torch: 64-bit tensors are left as they are (and refused below)
         x, weight, bias = (t if t is None or t.dtype == torch.float64 else t.to(dtype) for t in (x, weight, bias))
     _dtype_code(x.dtype, "linear")
+    if packed is None and share:
+        packed = _carried(given)
     if packed is not None:
         _require_same_device(packed.values, x.device, "linear: packed")
         if packed.shape != tuple(x.shape):
@@ -684,7 +686,7 @@ class Linear(nn.Linear):
     layers that read it."""
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return _linear(x, self.weight, self.bias, _carried(x), share=True)
+        return _linear(x, self.weight, self.bias, None, share=True)
 
 
 def pack_activations(module: nn.Module) -> nn.Module:
