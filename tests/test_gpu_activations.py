@@ -712,6 +712,54 @@ def test_captured_steps_replay(device):
                 assert_bits_equal(a, b)
 
 
+def test_graphed_callables(device):
+    """torch's own capture of a module, forward and backward apart."""
+    model = A.pack_activations(small_block(torch.bfloat16, device))
+    again = A.pack_activations(small_block(torch.bfloat16, device))
+    sample = torch.zeros(130, 192, dtype=torch.bfloat16, device=device, requires_grad=True)
+    graphed = torch.cuda.make_graphed_callables(model, (sample,))
+    for k in range(4):
+        x = randn(k, 130, 192, dtype=torch.bfloat16).to(device).requires_grad_()
+        g = randn(k + 9, 130, 100, dtype=torch.bfloat16).to(device)
+        out = graphed(x)
+        got = [t.clone() for t in torch.autograd.grad(out, [x, *model.parameters()], g)]
+        out = out.detach().clone()
+        torch.cuda.synchronize()
+        plain = again(x)
+        want = torch.autograd.grad(plain, [x, *again.parameters()], g)
+        assert_bits_equal(out, plain)
+        for a, b in zip(got, want):
+            assert_bits_equal(a, b)
+
+
+def test_captured_layers_on_two_streams(device):
+    """A capture that forks: the layer reads the norm's rows on the other stream, in every replay."""
+    norm, lin = A.RMSNorm(256).to(device), A.Linear(256, 16).to(device)
+    x = torch.zeros(40, 256, device=device)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        lin(norm(x))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = norm(x)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            out = lin(y)
+        torch.cuda.current_stream().wait_stream(side)
+        values, result = out.grad_fn.saved_tensors[1], out.detach()
+        assert values.data_ptr() == getattr(y, A._CARRIED).packed.values.data_ptr()
+        del y, out
+    for k in range(3):
+        x.copy_(randn(k, 40, 256))
+        graph.replay()
+        torch.cuda.synchronize()
+        plain = norm(x)
+        assert_bits_equal(result, lin(plain))
+        assert_bits_equal(values.view(torch.uint8), getattr(plain, A._CARRIED).packed.values.view(torch.uint8))
+
+
 # --- autograd, modules and the wrappers -----------------------------------------------------------
 
 
@@ -901,6 +949,23 @@ def test_a_norms_output_saves_and_loads_as_a_tensor(device):
     again = torch.load(file, weights_only=True)
     assert torch.equal(again, y)
     assert_bits_equal(layer(again), layer(y))
+
+
+def test_packed_rows_saved_on_the_host_and_modules_with_hooks(device):
+    x, g = randn(1, 33, 192).to(device), randn(2, 33, 100).to(device)
+    model = A.pack_activations(small_block(torch.float32, device))
+    want = torch.autograd.grad(model(x), list(model.parameters()), g)
+    with torch.autograd.graph.save_on_cpu():
+        out = model(x)
+    got = torch.autograd.grad(out, list(model.parameters()), g)
+    for m in model:
+        m.register_full_backward_hook(lambda *a: None)  # its inputs and outputs are views then
+        m.register_forward_hook(lambda *a: None)
+    inp = x.clone().requires_grad_()
+    hooked = torch.autograd.grad(model(inp), list(model.parameters()), g)
+    for a, b, c in zip(got, hooked, want):
+        assert_bits_equal(a, c)
+        assert_bits_equal(b, c)
 
 
 def test_input_buffers_are_packed_by_every_layer(device):
