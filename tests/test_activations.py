@@ -316,6 +316,17 @@ def test_weight_gradients_of_more_tiles_than_a_launch_holds_are_refused():
     assert rc == -2 and b"tiles" in lib.tft_last_error()
 
 
+@pytest.mark.parametrize("rows,out_features,features,dtype,tile,tiles,pieces", [
+    (8192, 4096, 4096, 1, 256, 256, 1), (8192, 1024, 4096, 1, 256, 64, 4), (4096, 2048, 2048, 2, 256, 64, 4),
+    (16384, 1000, 1000, 0, 256, 16, 16), (4096, 1024, 4096, 1, 128, 256, 2), (1024, 768, 768, 1, 128, 36, 4),
+    (1000, 1008, 768, 0, 128, 48, 5)])
+def test_how_weight_gradients_are_cut(rows, out_features, features, dtype, tile, tiles, pieces):
+    """The pieces that the figures beside the kernel speak of, by the workspace that they take."""
+    got = _native.lib().tft_linear_weight_grad_workspace(4096, rows, out_features, features, out_features,
+                                                         (features + 15) // 16 * 16, dtype)
+    assert got == (tiles * pieces * tile * tile * 4 if pieces > 1 else 0)
+
+
 # --- modules ------------------------------------------------------------------------------------
 
 

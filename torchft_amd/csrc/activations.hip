@@ -305,7 +305,8 @@ __device__ inline void dequantise(const u32x2& q, float scale, float (&v)[8]) {
   }
 }
 
-// n / d for n < 2^31 by a multiplication (d >= 1)
+// n / d for n < 2^31 by a multiplication (d >= 1): Granlund and Montgomery, "Division by invariant
+// integers using multiplication", 1994
 struct Divider {
   uint32_t d, magic, shift;
 };
@@ -339,7 +340,7 @@ constexpr int kPackBlocks = kPackThreads / 16 * kPackUnroll;  // blocks per work
 constexpr int kUnpackBlocks = kPackThreads / 16 * kUnpackUnroll;
 
 // Bound by memory: an element is read once and one byte written.  8192 x 14336 bf16 (353 MB)
-// takes 54 us, 6.5 TB/s; two or one blocks a lane instead of four 55 and 61 us.
+// takes 54-55 us, 6.4-6.5 TB/s; two or one blocks a lane instead of four 55 and 61 us.
 template <typename T, bool S>
 __global__ __launch_bounds__(kPackThreads) void pack_kernel(PackArgs a) {
   const int lane = threadIdx.x & 15;
@@ -443,8 +444,12 @@ struct NormArgs {
 // 512 features are one wavefront's, four rows to a workgroup and no barrier (Four); longer rows
 // take a workgroup of as many wavefronts as it has 512 features, from 8192 on twice as many
 // features a lane (C = 2).  One chunk of eight features a lane keeps the most wavefronts, and so
-// the most loads, in flight: 16384 x 4096 bf16 with a residual (604 MB) takes 99 us, 6.1 TB/s, with
-// eight wavefronts of one chunk, 101 with four of two, 104 with two of four.
+// the most loads, in flight: 16384 x 4096 bf16 with a residual (604 MB) takes 99 us at its least
+// (median 103, 5.9 TB/s) with eight wavefronts of one chunk, 101 with four of two, 104 with two of
+// four; without packing (537 MB) 90 and 94.  4096 x 14336 (C = 2, 528 MB): 94 us.  Rows much
+// shorter than 512 features leave lanes idle: at 128 features 16 of 64 work, and 262144 x 128 without
+// a residual (171 MB) takes 82-99 us, where its bytes alone would take 26.  A call of a few
+// megabytes is 3 us and its bytes: 5001 x 1000 fp16 with a residual (45 MB) 11.7 us.
 template <typename T, bool Four, int C, bool S>
 __global__ __launch_bounds__(Four ? 256 : 1024) void norm_kernel(NormArgs a) {
   const int kTeam = Four ? 64 : blockDim.x;
@@ -548,7 +553,9 @@ struct NormBackArgs {
 // weight gradient of its rows in registers; column_reduce_kernel adds the workgroups' partial
 // sums in a fixed order.  A row is asked for while the one before it is worked on: few rows are
 // in flight, because every workgroup leaves a partial sum of a whole row behind.  8192 x 4096 bf16
-// with grad_h (235 MB) takes 39 us, 6.0 TB/s, and 4.7 for the partial sums; without asking ahead 69.
+// with grad_h (235 MB) takes 39-43 us, 6.0-5.5 TB/s, and 4.7 for the partial sums; without asking ahead
+// 69.  4096 x 14336 (C = 2: without asking ahead, 411 MB) takes 94 and 6.7, 262144 x 128 (171 MB; idle
+// lanes as in norm_kernel, and 2048 wavefronts on the whole chip) 114 and 4.8.
 template <typename T, bool Four, int C>
 __global__ __launch_bounds__(Four ? 256 : 1024) void norm_back_kernel(NormBackArgs a) {
   constexpr int kRows = Four ? 4 : 1;
@@ -686,7 +693,9 @@ __global__ __launch_bounds__(1024) void column_reduce_kernel(const float* partia
 }
 
 // Partial column sums of a [rows, columns] matrix: 256 lanes of eight columns, rows
-// blockIdx.y, + gridDim.y, ..., four of them in flight.
+// blockIdx.y, + gridDim.y, ..., four of them in flight.  Bound by memory, with few loads in flight as
+// for the norm's gradients: 8192 x 14336 bf16 (235 MB) takes 49 us, 4.8 TB/s, and 4.8 for the partial
+// sums; 8192 x 4096 13.3 and 4.0.
 template <typename T>
 __global__ __launch_bounds__(256) void column_sum_kernel(const void* x, float* partial, uint32_t rows,
                                                          int64_t columns, int64_t stride) {
@@ -1377,9 +1386,9 @@ uint32_t column_sum_groups(int64_t rows, int64_t columns) {
 }
 
 // Partial tiles that fit the XCDs' L2 together are written past it: the kernel's end would wait for
-// their write-back (1000 tokens, 1001 x 768 fp32, 16 MB: 27 us so, 30 through L2; 1024, 768 x 768
-// bf16, 7 MB: 15.3 and 16.3).  More of them are written back while the kernel runs, and the join
-// finds the rest in the cache (8192, 1024 x 4096, 67 MB: 80.6 and 77.2).
+// their write-back (1000 tokens, 1001 x 768 fp32, 16 MB: 27.5 us so, 29.4 through L2; 1024, 768 x 768
+// bf16, 9 MB: 15.5 and 16.6).  More of them are written back while the kernel runs, and the join
+// finds the rest in the cache (8192, 1024 x 4096, 67 MB: 80.7 and 77.3).
 constexpr int64_t kL2Bytes = 32ll << 20;
 
 // How a weight gradient is cut.
@@ -1411,9 +1420,11 @@ double wgrad_time(bool large, int64_t tiles, int64_t steps, int products, int64_
 
 // Large tiles read LDS less per product and small ones fill the chip with less; which of them, and
 // how many pieces, is the least of the times above.  Measured, us, large tiles in their best number
-// of pieces / small ones in theirs: 8192 tokens, 4096 x 4096 bf16 225 (1) / 306 (2); 8192,
-// 1024 x 4096 80 (4) / 88 (2); 4096, 2048 x 2048 fp16 80 (4) / 90 (2); 1024, 768 x 768 bf16
-// 21 (5) / 15 (3); 1000, 1001 x 768 fp32 31 (10) / 28 (3).
+// of pieces / small ones in theirs: 8192 tokens, 4096 x 4096 bf16 219 (1) / 290 (1); 8192,
+// 1024 x 4096 77 (4) / 85 (2); 4096, 2048 x 2048 fp16 78 (4) / 87 (2); 16384, 1000 x 1000 fp32 103 (16) /
+// 117 (8); 4096, 1024 x 4096 bf16 51 (3) / 49 (1), where small ones in 2 are taken (51); 1024, 768 x 768
+// bf16 18 (6) / 14.3 (3), where 4 are taken (15.1); 1000, 1001 x 768 fp32 31 (7) / 26 (4), where 5 are
+// taken (27.7): the estimate is up to 6 % off the best.
 WgradPlan plan_wgrad(int64_t rows, int64_t out_features, int64_t features, int64_t grad_stride,
                      int dtype, bool aligned) {
   WgradPlan p{};
