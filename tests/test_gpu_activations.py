@@ -1065,6 +1065,15 @@ def test_giving_a_norms_output_other_storage(device):
     gw, = torch.autograd.grad((lin(y) * g).sum(), (lin.weight,))
     assert_bits_equal(gw, A.linear_weight_grad(g, A.pack(y.detach())))
     assert not torch.equal(kept, y)
+    for made in (A.RMSNorm(64).to(device), torch.relu):  # the same address, turned around
+        y = made(randn(1, 64, 64).to(device).requires_grad_())
+        first = A.Linear(64, 8).to(device)
+        out = first(y)
+        y.data = y.data.t()
+        g = randn(2, 64, 8).to(device)
+        gw, = torch.autograd.grad((first(y) * g).sum(), (first.weight,))
+        assert_bits_equal(gw, A.linear_weight_grad(g, A.pack(y.detach().contiguous())))
+        del out
 
 
 def test_packed_rows_outlive_the_stream_that_reads_them(device):

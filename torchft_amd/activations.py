@@ -553,7 +553,7 @@ def _linear(
         # as torch: 64-bit tensors are left as they are (and refused below)
         x, weight, bias = (t if t is None or t.dtype == torch.float64 else t.to(dtype) for t in (x, weight, bias))
     _dtype_code(x.dtype, "linear")
-    if packed is None and share:
+    if packed is None and share and torch.is_grad_enabled():
         packed = _carried(given)
     if packed is not None:
         _require_same_device(packed.values, x.device, "linear: packed")
@@ -579,8 +579,8 @@ def _linear(
 # A norm's output carries its packed form with it, so that the linear layers reading it share one
 # copy.  An output that was written to since or given other storage, or whose norm's weight was
 # written to, or a tensor made from it (all its rows in another shape apart), does not have it and is
-# packed by the layer.  Neither is the form of an output used by a graph capture that the norm was not part of: the replays would read
-# rows that nobody packs again.
+# packed by the layer.  Nor is it used by a graph capture that the norm was not part of: the replays
+# would read rows that nobody packs again.
 _CARRIED = "_torchft_amd_packed"
 
 
@@ -608,25 +608,23 @@ def _carried(x: torch.Tensor) -> Optional[PackedActivation]:
     """x's packed form, where x carries one and it is still x's, or where x is a view of all rows of
     a tensor that does."""
     c = getattr(x, _CARRIED, None)
-    if c is None and torch.is_grad_enabled() and x._is_view():
-        whole = x._base
-        c = getattr(whole, _CARRIED, None)
-        if c is not None and not (x.dim() and x.shape[-1:] == whole.shape[-1:] and x.numel() == whole.numel()
-                                  and x.dtype == whole.dtype and x.is_contiguous() and whole.is_contiguous()):
-            return None
-    if type(c) is not _Carried or c.version != x._version or c.address != x.data_ptr() \
-            or not c.packed._scale_is_as_packed():
+    if c is None and x._is_view():
+        c = getattr(x._base, _CARRIED, None)
+    if type(c) is not _Carried or c.version != x._version or c.address != x.data_ptr():
+        return None
+    p = c.packed
+    if x.shape[-1:] != p.shape[-1:] or x.numel() != math.prod(p.shape) or x.dtype != p.dtype \
+            or not x.is_contiguous() or not p._scale_is_as_packed():
         return None
     stream = _raw_stream(x.device.index)
     capture = _native.lib().tft_capture_id(stream)
     if capture != c.capture or capture == _UNKNOWN_CAPTURE:
         return None
     if stream != c.stream:  # the caller has seen to x; nobody but us knows of what lies behind it
-        c.packed.record_stream(torch.cuda.current_stream(x.device))
-    if c.packed.shape != tuple(x.shape):
-        p = c.packed
-        return _trusted(p.values, p.exponents, p.features, p.column_scale, tuple(x.shape), p.dtype)
-    return c.packed
+        p.record_stream(torch.cuda.current_stream(x.device))
+    if p.shape != tuple(x.shape):
+        p = _trusted(p.values, p.exponents, p.features, p.column_scale, tuple(x.shape), p.dtype)
+    return p
 
 
 # Several layers may read an activation that no norm of ours made.  The first of them packs it, and
@@ -644,6 +642,8 @@ class _Shared(NamedTuple):
     dtype: torch.dtype  # what was packed: the activation, or what autocast made of it
     version: int  # of the activation
     address: int
+    strides: Tuple[int, ...]
+    shape: Tuple[int, ...]
     capture: int
     stream: int
 
@@ -657,7 +657,7 @@ def _shared(given: torch.Tensor, x: torch.Tensor) -> Optional[PackedActivation]:
     capture = _native.lib().tft_capture_id(stream)
     if capture == _UNKNOWN_CAPTURE:
         return None
-    now = (x.dtype, given._version, given.data_ptr(), capture, stream)
+    now = (x.dtype, given._version, given.data_ptr(), given.stride(), tuple(given.shape), capture, stream)
     s = getattr(given, _SHARED, None)
     if type(s) is _Shared and s[2:] == now:
         values, exponents = s.values(), s.exponents()
