@@ -331,6 +331,17 @@ def test_norm_of_nothing(device):
     assert gx.shape == (0, 20) and torch.equal(gw.cpu(), torch.zeros(20))
 
 
+def test_norm_of_rows_without_features(device):
+    """Nothing that a call returns is left as the allocator found it."""
+    used = torch.full((1 << 16,), 7.0, device=device)
+    del used
+    y, h, p, rstd = A.rms_norm_forward(torch.zeros(5, 0, device=device), torch.zeros(0, device=device))
+    assert y.shape == h.shape == p.unpack().shape == (5, 0)
+    assert torch.isnan(rstd).all()  # 0 / 0
+    gx, gw = A.rms_norm_backward(y, p, rstd)
+    assert gx.shape == (5, 0) and gw.shape == (0,)
+
+
 # --- weight gradient ----------------------------------------------------------------------------
 
 PARTS = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}

@@ -321,6 +321,8 @@ def rms_norm_forward(
     y = _contiguous_like(x)
     h = x if residual is None else _contiguous_like(x)
     rstd = torch.empty(rows, dtype=torch.float32, device=device)
+    if features == 0:
+        rstd.fill_(math.nan)  # the mean of nothing; the kernel has no rows to write it for
     values = exponents = packed = None
     if pack:
         values, exponents = _buffers(rows, features, device)
