@@ -300,10 +300,10 @@ int tft_column_sum(void* out, void* workspace, int64_t workspace_bytes, const vo
 /* grad_weight[o][f] = column_scale[f] * sum over rows t of grad_out[t][o] * packed[t][f]
  * (no scale where it is NULL), [out_features, features] contiguous and starting at a multiple of
  * 16 bytes.  Products of bf16 numbers that add up to the operands exactly (to fp32 gradients down
- * to 2^-133), sums in fp32, rounded once.  The workspace depends on the address of grad_out by its alignment only.  Rows of grad_out
- * that are read as they lie (16-byte aligned, a whole number of eights) have to start less than
- * 2^25 bytes apart, and out_features and pitch have to be less than that in bytes; else
- * TFT_ERR_UNSUPPORTED. */
+ * to 2^-133), sums in fp32, rounded once.  The workspace depends on the address of grad_out by its
+ * alignment only.  Rows of grad_out that are read as they lie (16-byte aligned, a whole number of
+ * eights) have to start less than 2^25 bytes apart, and out_features and pitch have to be less than
+ * that in bytes; else TFT_ERR_UNSUPPORTED. */
 int64_t tft_linear_weight_grad_workspace(const void* grad_out, int64_t rows, int64_t out_features,
                                          int64_t features, int64_t grad_row_stride, int64_t pitch,
                                          int dtype);

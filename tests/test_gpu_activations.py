@@ -9,7 +9,7 @@ from torch import nn
 
 from helpers import assert_bits_equal
 from oracle import packed_activations as O
-from torchft_amd import PackedActivation, PureDistributedDataParallel, _native
+from torchft_amd import PackedActivation, PureDistributedDataParallel
 from torchft_amd import activations as A
 
 pytestmark = pytest.mark.gpu
@@ -413,7 +413,7 @@ def test_weight_gradient_of_large_layers(device, rows, out_features, features, d
 def plan_of(device, rows, out_features, features, dtype):
     """Pieces' workspace of a weight gradient whose rows are read as they lie."""
     d = torch.empty(16, device=device, dtype=dtype)
-    return _native.lib().tft_linear_weight_grad_workspace(d.data_ptr(), rows, out_features, features, out_features,
+    return A._native.lib().tft_linear_weight_grad_workspace(d.data_ptr(), rows, out_features, features, out_features,
                                                           (features + 15) // 16 * 16, A._DTYPES[dtype])
 
 
@@ -663,7 +663,7 @@ def test_a_captured_layer_packs_what_its_replays_read(device):
         lin(norm(randn(1, 6, 130).to(device)))
     torch.cuda.current_stream().wait_stream(side)
     y = norm(randn(1, 6, 130).to(device))
-    assert _native.lib().tft_capture_id(torch.cuda.current_stream().cuda_stream) == 0
+    assert A._native.lib().tft_capture_id(torch.cuda.current_stream().cuda_stream) == 0
     kept, ids = [], []
     graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
     for graph in graphs:
@@ -671,7 +671,7 @@ def test_a_captured_layer_packs_what_its_replays_read(device):
             out = lin(y)
             z = norm(y)
             again = lin(z)  # the graph's own norm packs for this one
-            ids.append(_native.lib().tft_capture_id(torch.cuda.current_stream().cuda_stream))
+            ids.append(A._native.lib().tft_capture_id(torch.cuda.current_stream().cuda_stream))
             kept.append((out.grad_fn.saved_tensors[1], again.grad_fn.saved_tensors[1]))
             assert kept[-1][1].data_ptr() == getattr(z, A._CARRIED).packed.values.data_ptr()
             del out, z, again

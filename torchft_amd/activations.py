@@ -155,7 +155,9 @@ class PackedActivation:
     """An activation in 8 bits: E4M3 ``values`` of [rows, features rounded up to 16] and biased
     ``exponents`` (uint8) of [rows, blocks of 128 features].  An element stands for
     ``value * 2 ** (exponent - 127)``, times ``column_scale`` of its feature where there is one
-    (a norm's weight).  ``shape`` is the packed tensor's and ``dtype`` its type."""
+    (a norm's weight, the live one: a write to it changes what the form stands for, and
+    :func:`linear` refuses the form from then on).  ``shape`` is the packed tensor's and ``dtype`` its
+    type."""
 
     __slots__ = ("values", "exponents", "features", "shape", "dtype", "column_scale", "_scale_version")
 
